@@ -386,6 +386,63 @@ int qie_gelu_erf_bf16(void* x, int64_t ld, int rows, int n, qie_stream_t stream)
 /* Qwen2MLP gating: y = bf16(bf16(silu(g)) * u) with [g | u] = gu[r][0..F) | gu[r][F..2F). */
 int qie_silu_mul_bf16(const void* gu, int64_t ldg, int rows, int F, void* y, int64_t ldy, qie_stream_t stream);
 
+/* ------------------------------------------------------------------ sequences and their cache
+ * Rotary positions, a paged cache of k and v, and the attention over packed sequences and over the
+ * cache: several prompts in one pass, and new tokens after what is cached of a prompt.
+ * Lengths, tables, positions and slots are device memory; values that do not fit (offsets outside
+ * [0, tokens], lengths outside the table, pages outside the pool) are clamped or skipped as said,
+ * never followed out of bounds. */
+
+/* Rotary positions with several axes. Pair i < pairs of a head turns by positions[axis[i]][row] *
+ * turns[i] full turns (64-bit product and fraction):
+ *   (x, y) <- bf16(x cos - y sin), bf16(y cos + x sin),
+ * (x, y) = elements (i, pairs + i), or (2i, 2i + 1) if interleaved; elements past 2 pairs pass
+ * through. x: the first of `heads` heads, head_stride elements apart, of each of `rows` rows;
+ * out: the same layout, x itself or memory apart from it. positions: int32 [axes], rows ldp apart;
+ * turns: [pairs] (theta^(-i/n) / 2 pi for the usual ladder); axis: [pairs], clamped to the axes.
+ * 4-byte aligned, even strides (16-byte rows and heads are the fast form); pairs <= 128. */
+int qie_rope_axes_bf16(const void* x, int64_t ldx, void* out, int64_t ldo, int rows, int heads, int head_dim,
+                       int head_stride, const int* positions, int64_t ldp, int axes, const double* turns,
+                       const int* axis, int pairs, int interleaved, qie_stream_t stream);
+
+/* The same rotation on rows [q heads | k heads | v heads] with the cache's write: q goes to q_out
+ * [rows][heads * head_dim] (qkv itself: in place), k (rotated) and v (as it is) to
+ * pages[slot / page_size][kv head][slot % page_size][head_dim] at slots[row], strides in elements,
+ * the same for k_pages and v_pages. A slot < 0 or past the pool is not stored; slots of one call
+ * are distinct. head_dim % 8 == 0, page_size a power of two in [16, 1024], 16-byte aligned rows. */
+int qie_rope_append_bf16(const void* qkv, int64_t ldx, void* q_out, int64_t ldo, int rows, int heads, int kv_heads,
+                         int head_dim, const int* positions, int64_t ldp, int axes, const double* turns,
+                         const int* axis, int pairs, int interleaved, void* k_pages, void* v_pages, int num_pages,
+                         int page_size, int64_t page_stride, int64_t page_head_stride, int64_t slot_stride,
+                         const int64_t* slots, qie_stream_t stream);
+
+/* Attention within each of `seqs` packed sequences: rows [cu_seqlens[b], cu_seqlens[b + 1]) of q
+ * [tokens][heads][head_dim] over the same rows of k, v [tokens][kv_heads][head_dim] (query head h
+ * reads kv head h / (heads / kv_heads)); causal: key j <= query i. fp32 softmax, P rounded to bf16
+ * for P.V. What a query does not see does not reach it, infinities and NaN included. Rows outside
+ * every sequence are left as they were. Strides in elements, multiples of 8; head_dim % 8 == 0,
+ * <= 128; scale > 0. */
+int qie_attention_packed_bf16(const void* q, int64_t ldq, int64_t hsq, const void* k, const void* v, int64_t ldk,
+                              int64_t hsk, const int* cu_seqlens, int seqs, int tokens, int heads, int kv_heads,
+                              int head_dim, int causal, float scale, void* out, int64_t ldo, int64_t hso,
+                              qie_stream_t stream);
+
+/* Attention of the newest tokens of each sequence over a paged cache that holds them already: rows
+ * [cu_seqlens[b], cu_seqlens[b + 1]) of q (one each if cu_seqlens is NULL) are the last n of the
+ * kv_lens[b] cached tokens; query i sees keys j <= kv_lens[b] - n + i. Key j is slot j % page_size of
+ * page page_table[b][j / page_size] (a page outside the pool reads as zeros), pages as in
+ * qie_rope_append_bf16. A row that sees no key is 0. Long rows are cut into chunks of keys whose
+ * fp32 partials meet in `workspace` (>= qie_attention_paged_workspace bytes, 16-byte aligned, not
+ * shared with a call that may run at the same time); the cuts go by a row's own sequence only. */
+int qie_attention_paged_workspace(int tokens, int heads, int head_dim, int table_width, int page_size,
+                                  int64_t* bytes);
+int qie_attention_paged_bf16(const void* q, int64_t ldq, int64_t hsq, const void* k_pages, const void* v_pages,
+                             int num_pages, int page_size, int64_t page_stride, int64_t page_head_stride,
+                             int64_t slot_stride, const int* page_table, int64_t ld_table, int table_width,
+                             const int* kv_lens, const int* cu_seqlens, int seqs, int tokens, int heads,
+                             int kv_heads, int head_dim, float scale, void* out, int64_t ldo, int64_t hso,
+                             void* workspace, int64_t workspace_bytes, qie_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

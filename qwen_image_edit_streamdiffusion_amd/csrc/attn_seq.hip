@@ -1,0 +1,492 @@
+// Attention of the prompt encoder's kind: sequences of different lengths in one launch, grouped
+// query heads, causal or full, k and v as packed token rows or in the pages of a cache.
+//
+//   o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i),  s_ij = scale q_i . k_j,  m_i = max_j s_ij
+// over the keys j that query i sees (lim_i of them: a prefix of its sequence); no key: o_i = 0.
+//
+// The G query heads that share a kv head are rows of one block: row r of sequence b is token r / G,
+// head hk G + r % G. K and V are then read once for G heads, a single token still fills G rows of a
+// matrix instruction, and a causal diagonal is G times narrower in rows.
+//
+// attn_seq_kernel: one work-group = 4 waves = 64 rows of one (sequence, kv head), 64-key tiles,
+// double-buffered in LDS by buffer_load ... lds. Per wave and tile, 16 rows:
+//   S^T = K Q^T (mfma 16x16x32, K rows by ds_read_b128 from an XOR-swizzled image, Q^T in registers)
+//   a lane holds 16 keys of one row: online softmax in log2 units (running max and sum in fp32, the
+//   rescale only when a max grows by more than 2^8), P rounded to bf16 for the second product
+//   O^T += V^T P^T (V^T by ds_read_b64_tr_b16; the S^T registers are the P^T operand)
+// Rows past a tile's last key come from the buffer's range check as zeros.
+#include "qie_common.h"
+
+namespace {
+
+constexpr int kBM = 64;      // rows of a work-group
+constexpr int kKB = 64;      // keys of a tile
+constexpr int kRowB = 256;   // LDS row: 128 elements, narrower heads leave zeros
+constexpr int kTile = kKB * kRowB;
+constexpr float kLow = -1e30f;     // "no key yet": finite, so that exp2(-inf - kLow) is 0 and not NaN
+constexpr float kRescale = 8.0f;   // lazy rescale threshold, log2 units
+
+struct SeqArgs {
+  const bf16_t* q;
+  int64_t ldq, hsq;
+  const bf16_t *k, *v;  // packed rows, or pages
+  int64_t ldk, hsk;     // row (slot) and head strides
+  bf16_t* out;
+  int64_t ldo, hso;
+  const int* cu;  // [B + 1] token offsets (nullptr: one token each)
+  int B, T, H, Hk, G, Dh;
+  int causal;
+  float c;  // scale * log2(e)
+  // paged
+  const int* table;
+  int64_t ldt, ps;
+  const int* kv_lens;
+  int width, pages, pshift;
+  // keys in chunks of ct tiles, fp32 partials (ct = 0: whole rows)
+  int ct, maxch;
+  float* ws;  // O [T * H][maxch][Dh], then (m, l) [T * H][maxch][2]
+};
+
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+__device__ __forceinline__ i32x4_t seq_rsrc(const bf16_t* base, int bytes) {
+  const uint64_t p = (uint64_t)base;
+  return i32x4_t{uni((int)(uint32_t)p), uni((int)(uint32_t)(p >> 32)), uni(bytes), 0x00020000};
+}
+// 1 KiB (4 LDS rows) straight from memory: lane i's 16 bytes go to dst + 16 i, zeros out of range
+__device__ __forceinline__ void seq_dma(const i32x4_t& r, const char QIE_LDS* dst, uint32_t voff) {
+  const int lds = uni((int)(uint32_t)(uintptr_t)dst);
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %0, %1, 0 offen lds"
+      :
+      : "v"(voff), "s"(r), "s"(lds)
+      : "memory", "m0");
+}
+
+// where item `idx` lies: sequence b, its first token, tokens n, keys kv, row block blk, key chunk ch
+struct Item {
+  int b, start, n, kv, blk, ch, nch;
+};
+
+template <bool PAGED>
+__device__ __forceinline__ void seq_span(const SeqArgs& a, int b, int& start, int& n, int& kv) {
+  int e;
+  if (a.cu) {
+    start = min(max(a.cu[b], 0), a.T);
+    e = min(max(a.cu[b + 1], start), a.T);
+  } else {
+    start = min(b, a.T);
+    e = min(b + 1, a.T);
+  }
+  n = e - start;
+  kv = PAGED ? min(max(a.kv_lens[b], 0), a.width << a.pshift) : n;
+}
+
+// The idx-th (row block, key chunk) over all sequences: a wave-wide scan of the sequences' counts.
+template <bool PAGED, int BM>
+__device__ __forceinline__ bool find_item(const SeqArgs& a, int idx, Item& it) {
+  const int lane = threadIdx.x & 63;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    int start = 0, n = 0, kv = 0, cnt = 0;
+    if (b0 + lane < a.B) {
+      seq_span<PAGED>(a, b0 + lane, start, n, kv);
+      cnt = (n * a.G + BM - 1) / BM;
+      if (a.ct) cnt *= max(1, (kv + a.ct * kKB - 1) / (a.ct * kKB));
+    }
+    int pre = cnt;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(pre, o, 64);
+      if (lane >= o) pre += u;
+    }
+    const unsigned long long hit = __ballot(pre > idx);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      it.b = uni(b0 + l);
+      it.start = uni(__shfl(start, l, 64));
+      it.n = uni(__shfl(n, l, 64));
+      it.kv = uni(__shfl(kv, l, 64));
+      const int j = idx - uni(__shfl(pre - cnt, l, 64));
+      it.nch = a.ct ? max(1, (it.kv + a.ct * kKB - 1) / (a.ct * kKB)) : 1;
+      const int nblk = (it.n * a.G + BM - 1) / BM;
+      it.blk = nblk - 1 - j / it.nch;  // the longest rows of a causal sequence first
+      it.ch = j % it.nch;
+      return true;
+    }
+    idx -= uni(__shfl(pre, 63, 64));
+  }
+  return false;
+}
+
+// bf16 pairs with an infinity or NaN among them
+__device__ __forceinline__ bool nonfinite(const u32x4_t w) {
+  const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= (ww[i] & 0x7f80u) == 0x7f80u || (ww[i] & 0x7f800000u) == 0x7f800000u;
+  return bad;
+}
+// kind 0: the finite values; 1 / 2 / 3: ones where +inf / -inf / NaN stands
+__device__ __forceinline__ bf16x8_t pick(bf16x8_t x, int kind) {
+  const u32x4_t w = __builtin_bit_cast(u32x4_t, x);
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
+    uint32_t r = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t e = (u >> (16 * h)) & 0xffffu;
+      const bool fin = (e & 0x7f80u) != 0x7f80u;
+      const bool hit = kind == 1 ? e == 0x7f80u : kind == 2 ? e == 0xff80u : !fin && (e & 0x7fu);
+      r |= (kind == 0 ? (fin ? e : 0u) : hit ? 0x3f80u : 0u) << (16 * h);
+    }
+    o[i] = r;
+  }
+  return __builtin_bit_cast(bf16x8_t, u32x4_t{o[0], o[1], o[2], o[3]});
+}
+
+template <bool PAGED, int NK>  // NK 32-wide steps of the head: head_dim <= 32 NK
+__global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
+  constexpr int ND = 2 * NK;  // 16-wide blocks of the output
+  __shared__ __attribute__((aligned(16))) char smem_raw[4 * kTile];  // K0 V0 K1 V1
+  char QIE_LDS* smem = (char QIE_LDS*)smem_raw;
+
+  const int hk = blockIdx.x % a.Hk;
+  Item it;
+  if (!find_item<PAGED, kBM>(a, blockIdx.x / a.Hk, it)) return;
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
+  const int g = lane >> 4, ql = lane & 15;
+  const int rows = it.n * a.G;
+  const int r = it.blk * kBM + wave * 16 + ql;
+  const int tok = min(r, rows - 1) / a.G, head = hk * a.G + min(r, rows - 1) % a.G;
+  // keys that a row sees; of the wave's first row and of the block's last one
+  const int off = it.kv - it.n;
+  const int lim = a.causal ? min(it.kv, max(off + tok + 1, 0)) : it.kv;
+  const int lim0 = uni(lim);
+  const int last = (min(rows, (it.blk + 1) * kBM) - 1) / a.G;
+  const int most = a.causal ? min(it.kv, max(off + last + 1, 0)) : it.kv;
+  const int ntot = (most + kKB - 1) / kKB;
+  const int t0 = a.ct ? it.ch * a.ct : 0;
+  const int t1 = a.ct ? min(ntot, t0 + a.ct) : ntot;
+  const bool whole = !a.ct || ntot <= a.ct;
+  if (t0 > 0 && t0 >= ntot) return;  // a causal block that ends before this chunk
+
+  bf16x8_t qf[NK];
+  const bf16_t* qr = a.q + (int64_t)(it.start + tok) * a.ldq + (int64_t)head * a.hsq;
+#pragma unroll
+  for (int ks = 0; ks < NK; ++ks) {
+    qf[ks] = bf16x8_t{};
+    if (32 * ks + 8 * g < a.Dh) qf[ks] = *(const bf16x8_t*)(qr + 32 * ks + 8 * g);
+  }
+
+  // ---- tiles by LDS-DMA: a piece is 4 rows; wave w takes pieces w, w + 4, ... of K and of V. The
+  // source chunk carries the XOR swizzle: K by the row, V by the row's low three bits, doubled
+  const int prow = lane >> 4, pch = lane & 15;
+  const int* table = PAGED ? a.table + (int64_t)it.b * a.ldt : nullptr;
+  auto dma = [&](int t, int buf) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const int r0 = (wave + 4 * p) * 4;
+      const int key = t * kKB + r0;
+      const int nrow = min(4, it.kv - key);
+      int64_t at;
+      bool ok = nrow > 0;
+      if constexpr (PAGED) {
+        const int id = ok ? table[key >> a.pshift] : 0;
+        ok = ok && id >= 0 && id < a.pages;
+        at = (int64_t)(ok ? id : 0) * a.ps + (int64_t)hk * a.hsk + (int64_t)(key & ((1 << a.pshift) - 1)) * a.ldk;
+      } else {
+        at = ok ? (int64_t)(it.start + key) * a.ldk + (int64_t)hk * a.hsk : 0;
+      }
+      const int bytes = ok ? (int)((nrow - 1) * a.ldk * 2) + a.Dh * 2 : 0;
+      const uint32_t ro = prow * (uint32_t)(a.ldk * 2);
+      const int row = r0 + prow;
+      const int ck = pch ^ (row & 15), cv = pch ^ ((row & 7) << 1);
+      seq_dma(seq_rsrc(a.k + at, bytes), smem + (2 * buf) * kTile + r0 * kRowB, ck * 8 < a.Dh ? ro + ck * 16 : 0x80000000u);
+      seq_dma(seq_rsrc(a.v + at, bytes), smem + (2 * buf + 1) * kTile + r0 * kRowB, cv * 8 < a.Dh ? ro + cv * 16 : 0x80000000u);
+    }
+  };
+
+  f32x4_t o[ND];
+#pragma unroll
+  for (int db = 0; db < ND; ++db) o[db] = f32x4_t{};
+  float m_run = kLow, l_run = 0.f;
+
+  __builtin_amdgcn_s_waitcnt(0);  // q has landed: from here on the counter is the tiles'
+  if (t0 < t1) dma(t0, 0);
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    if (t + 1 < t1) {
+      dma(t + 1, buf ^ 1);
+      asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+    const char QIE_LDS* kt = smem + (2 * buf) * kTile;
+    const char QIE_LDS* vt = kt + kTile;
+    f32x4_t s[4];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      s[kb] = f32x4_t{};
+#pragma unroll
+      for (int ks = 0; ks < NK; ++ks) {
+        const bf16x8_t A = *(const bf16x8_t QIE_LDS*)(kt + (kb * 16 + ql) * kRowB + (((4 * ks + g) ^ ql) << 4));
+        s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, qf[ks], s[kb], 0, 0, 0);
+      }
+    }
+    const int kv0 = t * kKB;
+    const bool masked = kv0 + kKB > lim0;
+    if (masked) {
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (kv0 + kb * 16 + 4 * g + i >= lim) s[kb][i] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[kb][i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    if (__any((mx - m_run) * a.c > kRescale)) {
+      const float m_new = fmaxf(m_run, mx);
+      const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * a.c);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < ND; ++db) o[db] *= alpha;
+    }
+    const float mc = m_run * a.c;
+    bf16x8_t pf[2];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], a.c, -mc));
+        l_run += p;
+        pf[kb >> 1][4 * (kb & 1) + i] = (__bf16)p;
+      }
+    // V^T fragment: lane's d = 16 db + ql, keys 32 k2 + 4 g + 0..3 and 16 further
+    auto vfrag = [&](int k2, int db) -> bf16x8_t {
+      const int row = 32 * k2 + 4 * g + (ql >> 2);
+      const int ch = (2 * db + ((ql & 3) >> 1)) ^ ((row & 7) << 1);
+      const char QIE_LDS* p0 = vt + row * kRowB + (ch << 4) + 8 * (ql & 1);
+      const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t QIE_LDS*)p0);
+      const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t QIE_LDS*)(p0 + 16 * kRowB));
+      return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    // 0 * inf and 0 * NaN: a masked key's V must not reach the rows that do not see it
+    bool bad = false;
+    if (masked) {
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+        for (int db = 0; db < ND; ++db) bad |= nonfinite(__builtin_bit_cast(u32x4_t, vfrag(k2, db)));
+      asm volatile("" ::: "memory");  // read again below: keeping all of them costs 64 registers
+    }
+    if (__builtin_expect(__any(bad), 0)) {
+      // the finite values as ever; then, where a row sees an infinity or NaN, that value itself
+#pragma unroll 1
+      for (int kind = 0; kind < 4; ++kind) {
+        asm volatile("" ::: "memory");
+        const float add = kind == 1 ? INFINITY : kind == 2 ? -INFINITY : __builtin_nanf("");
+#pragma unroll
+        for (int db = 0; db < ND; ++db) {
+          f32x4_t n = kind ? f32x4_t{} : o[db];
+#pragma unroll
+          for (int k2 = 0; k2 < 2; ++k2) {
+            bf16x8_t see = pf[k2];
+            if (kind)
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                see[i] = (__bf16)(kv0 + 32 * k2 + 16 * (i >> 2) + 4 * g + (i & 3) < lim ? 1.f : 0.f);
+            n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pick(vfrag(k2, db), kind), see, n, 0, 0, 0);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[db][i] = kind == 0 ? n[i] : n[i] > 0.f ? o[db][i] + add : o[db][i];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+        for (int db = 0; db < ND; ++db)
+          o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vfrag(k2, db), pf[k2], o[db], 0, 0, 0);
+    }
+    // this tile's reads are done: its buffer is free for the one after the next
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+
+  float l = l_run + __shfl_xor(l_run, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (r >= rows) return;
+  if (!whole) {
+    const int64_t pi = ((int64_t)(it.start + tok) * a.H + head) * a.maxch + it.ch;
+    float* po = a.ws + pi * a.Dh;
+    float* pml = a.ws + (int64_t)a.T * a.H * a.maxch * a.Dh + pi * 2;
+#pragma unroll
+    for (int db = 0; db < ND; ++db)
+      if (16 * db + 4 * g < a.Dh) *(f32x4_t*)(po + 16 * db + 4 * g) = o[db];
+    if (g == 0) *(f32x2_t*)pml = f32x2_t{m_run, l};
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;  // no key seen: o is 0 as well
+  bf16_t* dst = a.out + (int64_t)(it.start + tok) * a.ldo + (int64_t)head * a.hso;
+#pragma unroll
+  for (int db = 0; db < ND; ++db)
+    if (16 * db + 4 * g < a.Dh)
+      *(u32x2_t*)(dst + 16 * db + 4 * g) = u32x2_t{pack2(o[db][0] * inv, o[db][1] * inv),
+                                                   pack2(o[db][2] * inv, o[db][3] * inv)};
+}
+
+// Joins the chunks of a row: o = sum_c w_c o_c / sum_c w_c l_c, w_c = exp2((m_c - max m) c). One wave a
+// (token, head); the rows that one chunk held are written already.
+template <bool PAGED>
+__global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + uni(threadIdx.x >> 6);
+  if (row >= (int64_t)a.T * a.H) return;
+  const int token = (int)(row / a.H), head = (int)(row - (int64_t)token * a.H);
+  // the sequence of this token: the last one that starts at or before it
+  int b = -1, start = 0, n = 0, kv = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    int s0 = 0, n0 = 0, k0 = 0;
+    if (b0 + lane < a.B) seq_span<PAGED>(a, b0 + lane, s0, n0, k0);
+    const unsigned long long hit = __ballot(b0 + lane < a.B && s0 <= token && token < s0 + n0);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      b = b0 + l;
+      start = uni(__shfl(s0, l, 64));
+      n = uni(__shfl(n0, l, 64));
+      kv = uni(__shfl(k0, l, 64));
+      break;
+    }
+  }
+  if (b < 0) return;  // behind the last sequence
+  // the row's block saw the keys of its last token: chunks as attn_seq_kernel cut them
+  const int r = (token - start) * a.G + head % a.G, blk = r / kBM;
+  const int last = (min(n * a.G, (blk + 1) * kBM) - 1) / a.G;
+  const int most = a.causal ? min(kv, max(kv - n + last + 1, 0)) : kv;
+  const int ntot = (most + kKB - 1) / kKB, nch = (ntot + a.ct - 1) / a.ct;
+  if (nch <= 1) return;
+  const float* pml = a.ws + (int64_t)a.T * a.H * a.maxch * a.Dh + row * a.maxch * 2;
+  const float* po = a.ws + row * a.maxch * a.Dh;
+  float mx = kLow;
+  for (int c = 0; c < nch; ++c) mx = fmaxf(mx, pml[2 * c]);
+  float l = 0.f, o0 = 0.f, o1 = 0.f;
+  const int d = 2 * lane;
+  for (int c = 0; c < nch; ++c) {
+    const float w = __builtin_amdgcn_exp2f((pml[2 * c] - mx) * a.c);
+    l = __builtin_fmaf(w, pml[2 * c + 1], l);
+    if (d < a.Dh) {
+      const f32x2_t v = *(const f32x2_t*)(po + (int64_t)c * a.Dh + d);
+      o0 = __builtin_fmaf(w, v[0], o0);
+      o1 = __builtin_fmaf(w, v[1], o1);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  if (d < a.Dh) *(uint32_t*)(a.out + (int64_t)token * a.ldo + (int64_t)head * a.hso + d) = pack2(o0 * inv, o1 * inv);
+}
+
+template <bool PAGED>
+int launch_seq(const SeqArgs& a, hipStream_t s) {
+  const int64_t rb = (int64_t)a.T * a.G / kBM + a.B;  // at least the row blocks of any lengths
+  const int64_t grid = rb * (a.ct ? a.maxch : 1) * a.Hk;
+  if (grid > INT32_MAX) return QIE_ERR_UNSUPPORTED;
+  if (a.Dh <= 64) attn_seq_kernel<PAGED, 2><<<(unsigned)grid, 256, 0, s>>>(a);
+  else if (a.Dh <= 96) attn_seq_kernel<PAGED, 3><<<(unsigned)grid, 256, 0, s>>>(a);
+  else attn_seq_kernel<PAGED, 4><<<(unsigned)grid, 256, 0, s>>>(a);
+  if (a.ct) attn_seq_join_kernel<PAGED><<<(unsigned)(((int64_t)a.T * a.H + 3) / 4), 256, 0, s>>>(a);
+  return qie_last_error();
+}
+
+constexpr int kChunkTiles = 8;  // 512 keys
+
+bool seq_common_ok(const void* q, int64_t ldq, int64_t hsq, const void* k, const void* v, int64_t ldk, int64_t hsk,
+                   int seqs, int tokens, int heads, int kv_heads, int head_dim, float scale, const void* out,
+                   int64_t ldo, int64_t hso) {
+  if (!(q && k && v && out && seqs > 0 && tokens >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0)) return false;
+  if (!(head_dim > 0 && head_dim <= 128 && head_dim % 8 == 0 && scale > 0.f && scale < INFINITY)) return false;
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16 != 0) return false;
+  if ((ldq | hsq | ldk | hsk | ldo | hso) % 8 != 0) return false;
+  if (ldq < 0 || hsq < 0 || ldk < head_dim || ldk > INT32_MAX / 16 || hsk < 0 || ldo < head_dim || hso < head_dim) return false;
+  return (int64_t)tokens * heads <= INT32_MAX / 2;
+}
+
+}  // namespace
+
+extern "C" int qie_attention_packed_bf16(const void* q, int64_t ldq, int64_t hsq, const void* k, const void* v,
+                                         int64_t ldk, int64_t hsk, const int* cu_seqlens, int seqs, int tokens,
+                                         int heads, int kv_heads, int head_dim, int causal, float scale, void* out,
+                                         int64_t ldo, int64_t hso, qie_stream_t stream) {
+  QIE_CHECK_ARG(seq_common_ok(q, ldq, hsq, k, v, ldk, hsk, seqs, tokens, heads, kv_heads, head_dim, scale, out, ldo, hso));
+  QIE_CHECK_ARG(cu_seqlens);
+  if (tokens == 0) return QIE_OK;
+  SeqArgs a{};
+  a.q = (const bf16_t*)q; a.ldq = ldq; a.hsq = hsq;
+  a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.ldk = ldk; a.hsk = hsk;
+  a.out = (bf16_t*)out; a.ldo = ldo; a.hso = hso;
+  a.cu = cu_seqlens;
+  a.B = seqs; a.T = tokens; a.H = heads; a.Hk = kv_heads; a.G = heads / kv_heads; a.Dh = head_dim;
+  a.causal = causal != 0;
+  a.c = scale * 1.4426950408889634f;
+  return launch_seq<false>(a, (hipStream_t)stream);
+}
+
+namespace {
+int paged_chunks(int table_width, int page_size) {
+  const int64_t tiles = ((int64_t)table_width * page_size + kKB - 1) / kKB;
+  return (int)((tiles + kChunkTiles - 1) / kChunkTiles);
+}
+}  // namespace
+
+extern "C" int qie_attention_paged_workspace(int tokens, int heads, int head_dim, int table_width, int page_size,
+                                             int64_t* bytes) {
+  QIE_CHECK_ARG(bytes && tokens >= 0 && heads > 0 && head_dim > 0 && table_width > 0 && page_size > 0);
+  QIE_CHECK_ARG((int64_t)table_width * page_size <= INT32_MAX / 2);
+  const int ch = paged_chunks(table_width, page_size);
+  *bytes = ch > 1 ? (int64_t)tokens * heads * ch * (head_dim + 2) * 4 : 0;
+  return QIE_OK;
+}
+
+extern "C" int qie_attention_paged_bf16(const void* q, int64_t ldq, int64_t hsq, const void* k_pages,
+                                        const void* v_pages, int num_pages, int page_size, int64_t page_stride,
+                                        int64_t page_head_stride, int64_t slot_stride, const int* page_table,
+                                        int64_t ld_table, int table_width, const int* kv_lens, const int* cu_seqlens,
+                                        int seqs, int tokens, int heads, int kv_heads, int head_dim, float scale,
+                                        void* out, int64_t ldo, int64_t hso, void* workspace, int64_t workspace_bytes,
+                                        qie_stream_t stream) {
+  QIE_CHECK_ARG(seq_common_ok(q, ldq, hsq, k_pages, v_pages, slot_stride, page_head_stride, seqs, tokens, heads,
+                              kv_heads, head_dim, scale, out, ldo, hso));
+  QIE_CHECK_ARG(page_table && kv_lens && (cu_seqlens || seqs == tokens) && num_pages > 0 && table_width > 0);
+  QIE_CHECK_ARG(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0);
+  QIE_CHECK_ARG(page_stride >= 0 && page_stride % 8 == 0 && ld_table >= table_width);
+  QIE_CHECK_ARG((int64_t)table_width * page_size <= INT32_MAX / 2);
+  int64_t need = 0;
+  const int rc = qie_attention_paged_workspace(tokens, heads, head_dim, table_width, page_size, &need);
+  if (rc) return rc;
+  QIE_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0));
+  if (tokens == 0) return QIE_OK;
+  SeqArgs a{};
+  a.q = (const bf16_t*)q; a.ldq = ldq; a.hsq = hsq;
+  a.k = (const bf16_t*)k_pages; a.v = (const bf16_t*)v_pages; a.ldk = slot_stride; a.hsk = page_head_stride;
+  a.out = (bf16_t*)out; a.ldo = ldo; a.hso = hso;
+  a.cu = cu_seqlens;
+  a.B = seqs; a.T = tokens; a.H = heads; a.Hk = kv_heads; a.G = heads / kv_heads; a.Dh = head_dim;
+  a.causal = 1;
+  a.c = scale * 1.4426950408889634f;
+  a.table = page_table; a.ldt = ld_table; a.ps = page_stride;
+  a.kv_lens = kv_lens;
+  a.width = table_width; a.pages = num_pages; a.pshift = __builtin_ctz(page_size);
+  if (need) {
+    a.ct = kChunkTiles;
+    a.maxch = paged_chunks(table_width, page_size);
+    a.ws = (float*)workspace;
+  }
+  return launch_seq<true>(a, (hipStream_t)stream);
+}

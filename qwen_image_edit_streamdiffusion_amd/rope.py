@@ -8,6 +8,7 @@ The reference invokes it through every pipeline call
 """
 from __future__ import annotations
 
+import math
 from typing import Sequence, Tuple
 
 import torch
@@ -44,3 +45,22 @@ def rope_tables(img_shapes, txt_len: int, device, axes=(16, 56, 56), theta: floa
     for a in (ia, ta):
         out += [torch.cos(a).contiguous().to(device), torch.sin(a).contiguous().to(device)]
     return tuple(out)
+
+
+# ---------------------------------------------------------------------------- turns and axes of ops.rope_axes
+def section_turns(sections: Sequence[int], theta: float, device="cuda") -> Tuple[torch.Tensor, torch.Tensor]:
+    """(turns float64, axis int32) of ``ops.rope_axes`` for one ladder of frequencies cut into runs:
+    pair i turns theta^(-i / pairs) / 2 pi of a full turn a step, run a of the pairs goes by axis a
+    (the language model's ``mrope_section``; one section is ordinary rotary)."""
+    n = sum(sections)
+    turns = float(theta) ** (-torch.arange(n, dtype=torch.float64) / n) / (2 * math.pi)
+    axis = torch.repeat_interleave(torch.arange(len(sections)), torch.tensor(list(sections)))
+    return turns.to(device), axis.to(torch.int32).to(device)
+
+
+def axes_turns(dims: Sequence[int], theta: float = 10000.0, device="cuda") -> Tuple[torch.Tensor, torch.Tensor]:
+    """(turns, axis) for a ladder of its own on every axis, dims[a] elements wide (the image
+    transformer's (16, 56, 56), interleaved; the vision tower's (40, 40))."""
+    turns = torch.cat([float(theta) ** (-torch.arange(0, d, 2, dtype=torch.float64) / d) for d in dims]) / (2 * math.pi)
+    axis = torch.cat([torch.full((d // 2,), a, dtype=torch.int32) for a, d in enumerate(dims)])
+    return turns.to(device), axis.to(device)
