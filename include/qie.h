@@ -434,8 +434,8 @@ int qie_attention_packed_bf16(const void* q, int64_t ldq, int64_t hsq, const voi
  * qie_rope_append_bf16. A row that sees no key is 0. Long rows are cut into chunks of keys whose
  * fp32 partials meet in `workspace` (>= qie_attention_paged_workspace bytes, 16-byte aligned, not
  * shared with a call that may run at the same time); the cuts go by a row's own sequence only. */
-int qie_attention_paged_workspace(int tokens, int heads, int head_dim, int table_width, int page_size,
-                                  int64_t* bytes);
+int qie_attention_paged_workspace(int tokens, int seqs, int heads, int kv_heads, int head_dim, int table_width,
+                                  int page_size, int64_t* bytes);
 int qie_attention_paged_bf16(const void* q, int64_t ldq, int64_t hsq, const void* k_pages, const void* v_pages,
                              int num_pages, int page_size, int64_t page_stride, int64_t page_head_stride,
                              int64_t slot_stride, const int* page_table, int64_t ld_table, int table_width,

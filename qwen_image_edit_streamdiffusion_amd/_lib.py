@@ -86,7 +86,7 @@ SIGNATURES = {
     "qie_rope_axes_bf16": [P, L, P, L, I, I, I, I, P, L, I, P, P, I, I, P],
     "qie_rope_append_bf16": [P, L, P, L, I, I, I, I, P, L, I, P, P, I, I, P, P, I, I, L, L, L, P, P],
     "qie_attention_packed_bf16": [P, L, L, P, P, L, L, P, I, I, I, I, I, I, F, P, L, L, P],
-    "qie_attention_paged_workspace": [I, I, I, I, I, POINTER(c_int64)],
+    "qie_attention_paged_workspace": [I, I, I, I, I, I, I, POINTER(c_int64)],
     "qie_attention_paged_bf16": [P, L, L, P, P, I, I, L, L, L, P, L, I, P, P, I, I, I, I, I, F, P, L, L, P, L, P],
 }
 _RESTYPES = {"qie_strerror": c_char_p}

@@ -1,0 +1,138 @@
+// Shared pieces of the attention over sequences (attn_seq.hip: 64-row blocks, joins and dispatch;
+// attn_seq_pp.hip: 256-row blocks): arguments, where a work-group's item lies, tile loads, and what
+// keeps infinities and NaN of masked keys away from the rows that do not see them.
+#pragma once
+#include "qie_common.h"
+
+struct SeqArgs {
+  const bf16_t* q;
+  int64_t ldq, hsq;
+  const bf16_t *k, *v;  // packed rows, or pages
+  int64_t ldk, hsk;     // row (slot) and head strides
+  bf16_t* out;
+  int64_t ldo, hso;
+  const int* cu;  // [B + 1] token offsets (nullptr: one token each)
+  int B, T, H, Hk, G, Dh;
+  int causal;
+  float c;  // scale * log2(e)
+  // paged
+  const int* table;
+  int64_t ldt, ps;
+  const int* kv_lens;
+  int width, pages, pshift;
+  // keys in chunks of ct tiles, fp32 partials (ct = 0: whole rows); rows of a block
+  int ct, maxch, bm;
+  float* ws;  // O [T * H][maxch][Dh], then (m, l) [T * H][maxch][2]
+};
+
+namespace {
+
+constexpr int kKB = 64;      // keys of a tile
+constexpr int kRowB = 256;   // LDS row: 128 elements, narrower heads leave zeros
+constexpr int kTile = kKB * kRowB;
+constexpr float kLow = -1e30f;     // "no key yet": finite, so that exp2(-inf - kLow) is 0 and not NaN
+constexpr float kRescale = 8.0f;   // lazy rescale threshold, log2 units
+
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+__device__ __forceinline__ i32x4_t seq_rsrc(const bf16_t* base, int bytes) {
+  const uint64_t p = (uint64_t)base;
+  return i32x4_t{uni((int)(uint32_t)p), uni((int)(uint32_t)(p >> 32)), uni(bytes), 0x00020000};
+}
+// 1 KiB (4 LDS rows) straight from memory: lane i's 16 bytes go to dst + 16 i, zeros out of range
+__device__ __forceinline__ void seq_dma(const i32x4_t& r, const char QIE_LDS* dst, uint32_t voff) {
+  const int lds = uni((int)(uint32_t)(uintptr_t)dst);
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %0, %1, 0 offen lds"
+      :
+      : "v"(voff), "s"(r), "s"(lds)
+      : "memory", "m0");
+}
+
+// where item `idx` lies: sequence b, its first token, tokens n, keys kv, row block blk, key chunk ch
+struct Item {
+  int b, start, n, kv, blk, ch, nch;
+};
+
+template <bool PAGED>
+__device__ __forceinline__ void seq_span(const SeqArgs& a, int b, int& start, int& n, int& kv) {
+  int e;
+  if (a.cu) {
+    start = min(max(a.cu[b], 0), a.T);
+    e = min(max(a.cu[b + 1], start), a.T);
+  } else {
+    start = min(b, a.T);
+    e = min(b + 1, a.T);
+  }
+  n = e - start;
+  kv = PAGED ? min(max(a.kv_lens[b], 0), a.width << a.pshift) : n;
+}
+
+// The idx-th (row block, key chunk) over all sequences: a wave-wide scan of the sequences' counts.
+template <bool PAGED, int BM>
+__device__ __forceinline__ bool find_item(const SeqArgs& a, int idx, Item& it) {
+  const int lane = threadIdx.x & 63;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    int start = 0, n = 0, kv = 0, cnt = 0;
+    if (b0 + lane < a.B) {
+      seq_span<PAGED>(a, b0 + lane, start, n, kv);
+      cnt = (n * a.G + BM - 1) / BM;
+      if (a.ct) cnt *= max(1, (kv + a.ct * kKB - 1) / (a.ct * kKB));
+    }
+    int pre = cnt;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(pre, o, 64);
+      if (lane >= o) pre += u;
+    }
+    const unsigned long long hit = __ballot(pre > idx);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      it.b = uni(b0 + l);
+      it.start = uni(__shfl(start, l, 64));
+      it.n = uni(__shfl(n, l, 64));
+      it.kv = uni(__shfl(kv, l, 64));
+      const int j = idx - uni(__shfl(pre - cnt, l, 64));
+      it.nch = a.ct ? max(1, (it.kv + a.ct * kKB - 1) / (a.ct * kKB)) : 1;
+      const int nblk = (it.n * a.G + BM - 1) / BM;
+      it.ch = j / nblk;               // neighbours read the same keys
+      it.blk = nblk - 1 - j % nblk;  // the longest rows of a causal sequence first
+      return true;
+    }
+    idx -= uni(__shfl(pre, 63, 64));
+  }
+  return false;
+}
+
+// bf16 pairs with an infinity or NaN among them
+__device__ __forceinline__ bool nonfinite(const u32x4_t w) {
+  const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= (ww[i] & 0x7f80u) == 0x7f80u || (ww[i] & 0x7f800000u) == 0x7f800000u;
+  return bad;
+}
+// the finite values of a fragment, 0 for the others
+__device__ __forceinline__ bf16x8_t finite(bf16x8_t x) {
+  const u32x4_t w = __builtin_bit_cast(u32x4_t, x);
+  uint32_t o[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((o[i] & 0x7f80u) == 0x7f80u) o[i] &= 0xffff0000u;
+    if ((o[i] & 0x7f800000u) == 0x7f800000u) o[i] &= 0xffffu;
+  }
+  return __builtin_bit_cast(bf16x8_t, u32x4_t{o[0], o[1], o[2], o[3]});
+}
+// an infinity or NaN of a value that the row sees (low or high half of a pair), else 0
+__device__ __forceinline__ float special(uint32_t w, int high, bool see) {
+  const float f = high ? hi_f(w) : lo_f(w);
+  return see && (__float_as_uint(f) & 0x7f800000u) == 0x7f800000u ? f : 0.f;
+}
+
+}  // namespace
+
+// attn_seq_pp.hip: blocks of kPPRows rows
+constexpr int kPPRows = 256;
+int qie_launch_seq_pp(const SeqArgs& a, bool paged, hipStream_t s);

@@ -15,138 +15,11 @@
 //   rescale only when a max grows by more than 2^8), P rounded to bf16 for the second product
 //   O^T += V^T P^T (V^T by ds_read_b64_tr_b16; the S^T registers are the P^T operand)
 // Rows past a tile's last key come from the buffer's range check as zeros.
-#include "qie_common.h"
+#include "attn_seq.h"
 
 namespace {
 
-constexpr int kBM = 64;      // rows of a work-group
-constexpr int kKB = 64;      // keys of a tile
-constexpr int kRowB = 256;   // LDS row: 128 elements, narrower heads leave zeros
-constexpr int kTile = kKB * kRowB;
-constexpr float kLow = -1e30f;     // "no key yet": finite, so that exp2(-inf - kLow) is 0 and not NaN
-constexpr float kRescale = 8.0f;   // lazy rescale threshold, log2 units
-
-struct SeqArgs {
-  const bf16_t* q;
-  int64_t ldq, hsq;
-  const bf16_t *k, *v;  // packed rows, or pages
-  int64_t ldk, hsk;     // row (slot) and head strides
-  bf16_t* out;
-  int64_t ldo, hso;
-  const int* cu;  // [B + 1] token offsets (nullptr: one token each)
-  int B, T, H, Hk, G, Dh;
-  int causal;
-  float c;  // scale * log2(e)
-  // paged
-  const int* table;
-  int64_t ldt, ps;
-  const int* kv_lens;
-  int width, pages, pshift;
-  // keys in chunks of ct tiles, fp32 partials (ct = 0: whole rows)
-  int ct, maxch;
-  float* ws;  // O [T * H][maxch][Dh], then (m, l) [T * H][maxch][2]
-};
-
-__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
-__device__ __forceinline__ i32x4_t seq_rsrc(const bf16_t* base, int bytes) {
-  const uint64_t p = (uint64_t)base;
-  return i32x4_t{uni((int)(uint32_t)p), uni((int)(uint32_t)(p >> 32)), uni(bytes), 0x00020000};
-}
-// 1 KiB (4 LDS rows) straight from memory: lane i's 16 bytes go to dst + 16 i, zeros out of range
-__device__ __forceinline__ void seq_dma(const i32x4_t& r, const char QIE_LDS* dst, uint32_t voff) {
-  const int lds = uni((int)(uint32_t)(uintptr_t)dst);
-  asm volatile(
-      "s_mov_b32 m0, %2\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %0, %1, 0 offen lds"
-      :
-      : "v"(voff), "s"(r), "s"(lds)
-      : "memory", "m0");
-}
-
-// where item `idx` lies: sequence b, its first token, tokens n, keys kv, row block blk, key chunk ch
-struct Item {
-  int b, start, n, kv, blk, ch, nch;
-};
-
-template <bool PAGED>
-__device__ __forceinline__ void seq_span(const SeqArgs& a, int b, int& start, int& n, int& kv) {
-  int e;
-  if (a.cu) {
-    start = min(max(a.cu[b], 0), a.T);
-    e = min(max(a.cu[b + 1], start), a.T);
-  } else {
-    start = min(b, a.T);
-    e = min(b + 1, a.T);
-  }
-  n = e - start;
-  kv = PAGED ? min(max(a.kv_lens[b], 0), a.width << a.pshift) : n;
-}
-
-// The idx-th (row block, key chunk) over all sequences: a wave-wide scan of the sequences' counts.
-template <bool PAGED, int BM>
-__device__ __forceinline__ bool find_item(const SeqArgs& a, int idx, Item& it) {
-  const int lane = threadIdx.x & 63;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    int start = 0, n = 0, kv = 0, cnt = 0;
-    if (b0 + lane < a.B) {
-      seq_span<PAGED>(a, b0 + lane, start, n, kv);
-      cnt = (n * a.G + BM - 1) / BM;
-      if (a.ct) cnt *= max(1, (kv + a.ct * kKB - 1) / (a.ct * kKB));
-    }
-    int pre = cnt;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(pre, o, 64);
-      if (lane >= o) pre += u;
-    }
-    const unsigned long long hit = __ballot(pre > idx);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      it.b = uni(b0 + l);
-      it.start = uni(__shfl(start, l, 64));
-      it.n = uni(__shfl(n, l, 64));
-      it.kv = uni(__shfl(kv, l, 64));
-      const int j = idx - uni(__shfl(pre - cnt, l, 64));
-      it.nch = a.ct ? max(1, (it.kv + a.ct * kKB - 1) / (a.ct * kKB)) : 1;
-      const int nblk = (it.n * a.G + BM - 1) / BM;
-      it.blk = nblk - 1 - j / it.nch;  // the longest rows of a causal sequence first
-      it.ch = j % it.nch;
-      return true;
-    }
-    idx -= uni(__shfl(pre, 63, 64));
-  }
-  return false;
-}
-
-// bf16 pairs with an infinity or NaN among them
-__device__ __forceinline__ bool nonfinite(const u32x4_t w) {
-  const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= (ww[i] & 0x7f80u) == 0x7f80u || (ww[i] & 0x7f800000u) == 0x7f800000u;
-  return bad;
-}
-// kind 0: the finite values; 1 / 2 / 3: ones where +inf / -inf / NaN stands
-__device__ __forceinline__ bf16x8_t pick(bf16x8_t x, int kind) {
-  const u32x4_t w = __builtin_bit_cast(u32x4_t, x);
-  uint32_t o[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t u = i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
-    uint32_t r = 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t e = (u >> (16 * h)) & 0xffffu;
-      const bool fin = (e & 0x7f80u) != 0x7f80u;
-      const bool hit = kind == 1 ? e == 0x7f80u : kind == 2 ? e == 0xff80u : !fin && (e & 0x7fu);
-      r |= (kind == 0 ? (fin ? e : 0u) : hit ? 0x3f80u : 0u) << (16 * h);
-    }
-    o[i] = r;
-  }
-  return __builtin_bit_cast(bf16x8_t, u32x4_t{o[0], o[1], o[2], o[3]});
-}
+constexpr int kBM = 64;  // rows of a work-group
 
 template <bool PAGED, int NK>  // NK 32-wide steps of the head: head_dim <= 32 NK
 __global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
@@ -290,25 +163,21 @@ __global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
       asm volatile("" ::: "memory");  // read again below: keeping all of them costs 64 registers
     }
     if (__builtin_expect(__any(bad), 0)) {
-      // the finite values as ever; then, where a row sees an infinity or NaN, that value itself
-#pragma unroll 1
-      for (int kind = 0; kind < 4; ++kind) {
+      // the finite values as ever, then what a row sees of the others
+#pragma unroll
+      for (int j = 0; j < 2 * ND; ++j) {
         asm volatile("" ::: "memory");
-        const float add = kind == 1 ? INFINITY : kind == 2 ? -INFINITY : __builtin_nanf("");
+        o[j % ND] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(finite(vfrag(j / ND, j % ND)), pf[j / ND], o[j % ND], 0, 0, 0);
+      }
+#pragma unroll 1
+      for (int j = 0; j < kKB; ++j) {
+        const char QIE_LDS* vr = vt + j * kRowB + 8 * (g & 1);
+        const bool see = kv0 + j < lim;
 #pragma unroll
         for (int db = 0; db < ND; ++db) {
-          f32x4_t n = kind ? f32x4_t{} : o[db];
+          const u32x2_t w = *(const u32x2_t QIE_LDS*)(vr + (((2 * db + (g >> 1)) ^ ((j & 7) << 1)) << 4));
 #pragma unroll
-          for (int k2 = 0; k2 < 2; ++k2) {
-            bf16x8_t see = pf[k2];
-            if (kind)
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                see[i] = (__bf16)(kv0 + 32 * k2 + 16 * (i >> 2) + 4 * g + (i & 3) < lim ? 1.f : 0.f);
-            n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pick(vfrag(k2, db), kind), see, n, 0, 0, 0);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[db][i] = kind == 0 ? n[i] : n[i] > 0.f ? o[db][i] + add : o[db][i];
+          for (int i = 0; i < 4; ++i) o[db][i] += special(i < 2 ? w.x : w.y, i & 1, see);
         }
       }
     } else {
@@ -369,8 +238,8 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
   }
   if (b < 0) return;  // behind the last sequence
   // the row's block saw the keys of its last token: chunks as attn_seq_kernel cut them
-  const int r = (token - start) * a.G + head % a.G, blk = r / kBM;
-  const int last = (min(n * a.G, (blk + 1) * kBM) - 1) / a.G;
+  const int r = (token - start) * a.G + head % a.G, blk = r / a.bm;
+  const int last = (min(n * a.G, (blk + 1) * a.bm) - 1) / a.G;
   const int most = a.causal ? min(kv, max(kv - n + last + 1, 0)) : kv;
   const int ntot = (most + kKB - 1) / kKB, nch = (ntot + a.ct - 1) / a.ct;
   if (nch <= 1) return;
@@ -393,19 +262,45 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
   if (d < a.Dh) *(uint32_t*)(a.out + (int64_t)token * a.ldo + (int64_t)head * a.hso + d) = pack2(o0 * inv, o1 * inv);
 }
 
+// Which kernel, and how keys are cut: by what the host knows, the token, sequence and head counts and
+// the longest cache that a table can hold (0: packed sequences, never cut).
+struct SeqPlan {
+  int bm, ct, maxch;
+};
+
+SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, int64_t table_keys) {
+  const int64_t tiles = (table_keys + kKB - 1) / kKB;
+  const int64_t blocks = (int64_t)tokens * (heads / kv_heads) / kPPRows;  // full 256-row blocks a kv head
+  SeqPlan p{kBM, 0, 1};
+  const bool pp = blocks >= seqs && blocks * kv_heads >= 64;
+  if (pp) p.bm = kPPRows;
+  const int ct = table_keys == 0 ? 0 : pp ? (blocks * kv_heads < 512 ? 32 : 0) : 8;
+  if (ct && tiles > ct) {
+    p.ct = ct;
+    p.maxch = (int)((tiles + ct - 1) / ct);
+  }
+  return p;
+}
+
 template <bool PAGED>
-int launch_seq(const SeqArgs& a, hipStream_t s) {
-  const int64_t rb = (int64_t)a.T * a.G / kBM + a.B;  // at least the row blocks of any lengths
-  const int64_t grid = rb * (a.ct ? a.maxch : 1) * a.Hk;
-  if (grid > INT32_MAX) return QIE_ERR_UNSUPPORTED;
-  if (a.Dh <= 64) attn_seq_kernel<PAGED, 2><<<(unsigned)grid, 256, 0, s>>>(a);
-  else if (a.Dh <= 96) attn_seq_kernel<PAGED, 3><<<(unsigned)grid, 256, 0, s>>>(a);
-  else attn_seq_kernel<PAGED, 4><<<(unsigned)grid, 256, 0, s>>>(a);
+int launch_seq(SeqArgs& a, const SeqPlan& p, hipStream_t s) {
+  a.bm = p.bm;
+  a.ct = p.ct;
+  a.maxch = p.maxch;
+  if (p.bm == kPPRows) {
+    const int rc = qie_launch_seq_pp(a, PAGED, s);
+    if (rc) return rc;
+  } else {
+    const int64_t rb = (int64_t)a.T * a.G / kBM + a.B;  // at least the row blocks of any lengths
+    const int64_t grid = rb * a.maxch * a.Hk;
+    if (grid > INT32_MAX) return QIE_ERR_UNSUPPORTED;
+    if (a.Dh <= 64) attn_seq_kernel<PAGED, 2><<<(unsigned)grid, 256, 0, s>>>(a);
+    else if (a.Dh <= 96) attn_seq_kernel<PAGED, 3><<<(unsigned)grid, 256, 0, s>>>(a);
+    else attn_seq_kernel<PAGED, 4><<<(unsigned)grid, 256, 0, s>>>(a);
+  }
   if (a.ct) attn_seq_join_kernel<PAGED><<<(unsigned)(((int64_t)a.T * a.H + 3) / 4), 256, 0, s>>>(a);
   return qie_last_error();
 }
-
-constexpr int kChunkTiles = 8;  // 512 keys
 
 bool seq_common_ok(const void* q, int64_t ldq, int64_t hsq, const void* k, const void* v, int64_t ldk, int64_t hsk,
                    int seqs, int tokens, int heads, int kv_heads, int head_dim, float scale, const void* out,
@@ -414,7 +309,7 @@ bool seq_common_ok(const void* q, int64_t ldq, int64_t hsq, const void* k, const
   if (!(head_dim > 0 && head_dim <= 128 && head_dim % 8 == 0 && scale > 0.f && scale < INFINITY)) return false;
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16 != 0) return false;
   if ((ldq | hsq | ldk | hsk | ldo | hso) % 8 != 0) return false;
-  if (ldq < 0 || hsq < 0 || ldk < head_dim || ldk > INT32_MAX / 16 || hsk < 0 || ldo < head_dim || hso < head_dim) return false;
+  if (ldq < 0 || hsq < 0 || ldk < head_dim || ldk > (1 << 23) || hsk < 0 || ldo < head_dim || hso < head_dim) return false;
   return (int64_t)tokens * heads <= INT32_MAX / 2;
 }
 
@@ -435,22 +330,15 @@ extern "C" int qie_attention_packed_bf16(const void* q, int64_t ldq, int64_t hsq
   a.B = seqs; a.T = tokens; a.H = heads; a.Hk = kv_heads; a.G = heads / kv_heads; a.Dh = head_dim;
   a.causal = causal != 0;
   a.c = scale * 1.4426950408889634f;
-  return launch_seq<false>(a, (hipStream_t)stream);
+  return launch_seq<false>(a, seq_plan(tokens, seqs, heads, kv_heads, 0), (hipStream_t)stream);
 }
 
-namespace {
-int paged_chunks(int table_width, int page_size) {
-  const int64_t tiles = ((int64_t)table_width * page_size + kKB - 1) / kKB;
-  return (int)((tiles + kChunkTiles - 1) / kChunkTiles);
-}
-}  // namespace
-
-extern "C" int qie_attention_paged_workspace(int tokens, int heads, int head_dim, int table_width, int page_size,
-                                             int64_t* bytes) {
-  QIE_CHECK_ARG(bytes && tokens >= 0 && heads > 0 && head_dim > 0 && table_width > 0 && page_size > 0);
-  QIE_CHECK_ARG((int64_t)table_width * page_size <= INT32_MAX / 2);
-  const int ch = paged_chunks(table_width, page_size);
-  *bytes = ch > 1 ? (int64_t)tokens * heads * ch * (head_dim + 2) * 4 : 0;
+extern "C" int qie_attention_paged_workspace(int tokens, int seqs, int heads, int kv_heads, int head_dim,
+                                             int table_width, int page_size, int64_t* bytes) {
+  QIE_CHECK_ARG(bytes && tokens >= 0 && seqs > 0 && heads > 0 && kv_heads > 0 && head_dim > 0 && table_width > 0 &&
+                page_size > 0 && (int64_t)table_width * page_size <= INT32_MAX / 2);
+  const SeqPlan p = seq_plan(tokens, seqs, heads, kv_heads, (int64_t)table_width * page_size);
+  *bytes = p.ct ? (int64_t)tokens * heads * p.maxch * (head_dim + 2) * 4 : 0;
   return QIE_OK;
 }
 
@@ -468,7 +356,7 @@ extern "C" int qie_attention_paged_bf16(const void* q, int64_t ldq, int64_t hsq,
   QIE_CHECK_ARG(page_stride >= 0 && page_stride % 8 == 0 && ld_table >= table_width);
   QIE_CHECK_ARG((int64_t)table_width * page_size <= INT32_MAX / 2);
   int64_t need = 0;
-  const int rc = qie_attention_paged_workspace(tokens, heads, head_dim, table_width, page_size, &need);
+  const int rc = qie_attention_paged_workspace(tokens, seqs, heads, kv_heads, head_dim, table_width, page_size, &need);
   if (rc) return rc;
   QIE_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0));
   if (tokens == 0) return QIE_OK;
@@ -483,10 +371,7 @@ extern "C" int qie_attention_paged_bf16(const void* q, int64_t ldq, int64_t hsq,
   a.table = page_table; a.ldt = ld_table; a.ps = page_stride;
   a.kv_lens = kv_lens;
   a.width = table_width; a.pages = num_pages; a.pshift = __builtin_ctz(page_size);
-  if (need) {
-    a.ct = kChunkTiles;
-    a.maxch = paged_chunks(table_width, page_size);
-    a.ws = (float*)workspace;
-  }
-  return launch_seq<true>(a, (hipStream_t)stream);
+  a.ws = (float*)workspace;
+  return launch_seq<true>(a, seq_plan(tokens, seqs, heads, kv_heads, (int64_t)table_width * page_size),
+                          (hipStream_t)stream);
 }

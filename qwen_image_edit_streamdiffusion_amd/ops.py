@@ -842,10 +842,11 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     return out
 
 
-def attention_paged_workspace_bytes(tokens: int, heads: int, head_dim: int, table_width: int, page_size: int) -> int:
+def attention_paged_workspace_bytes(tokens: int, seqs: int, heads: int, kv_heads: int, head_dim: int,
+                                    table_width: int, page_size: int) -> int:
     """Bytes that ``attention_paged(..., workspace=)`` needs (0: none)."""
     n = ctypes.c_int64(0)
-    _lib.call("qie_attention_paged_workspace", tokens, heads, head_dim, table_width, page_size, ctypes.byref(n))
+    _lib.call("qie_attention_paged_workspace", tokens, seqs, heads, kv_heads, head_dim, table_width, page_size, ctypes.byref(n))
     return n.value
 
 
@@ -877,7 +878,7 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ldq, hsq = _heads3(q, "q")
     if T == 0:
         return out
-    need = attention_paged_workspace_bytes(T, H, Dh, W, P)
+    need = attention_paged_workspace_bytes(T, B, H, Hk, Dh, W, P)
     if need and workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     have = 0 if workspace is None else workspace.numel() * workspace.element_size()

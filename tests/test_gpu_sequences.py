@@ -474,7 +474,7 @@ def test_captured_steps_replay():
         q = ops.rope_append(x, H, Hk, Dh, pos, turns, axis, kp, vp, slots, out=out)
         return ops.attention_paged(q.view(B, H, Dh), kp, vp, table, lens, workspace=ws)
 
-    nb = ops.attention_paged_workspace_bytes(B, H, Dh, W, P)
+    nb = ops.attention_paged_workspace_bytes(B, B, H, Hk, Dh, W, P)
     assert nb > 0
     graphs = []
     for _ in range(2):

@@ -93,6 +93,6 @@ def test_entry_points_refuse_on_the_host(lib):
                          dict(ws=20)):
         assert paged(**kw) == -1, kw
     n = ctypes.c_int64(-1)
-    assert lib.qie_attention_paged_workspace(4, 4, 128, 1, 16, ctypes.byref(n)) == 0 and n.value == 0
-    assert lib.qie_attention_paged_workspace(4, 4, 128, 4096, 16, ctypes.byref(n)) == 0 and n.value > 0
-    assert lib.qie_attention_paged_workspace(4, 4, 128, 4096, 16, None) == -1
+    assert lib.qie_attention_paged_workspace(4, 1, 4, 1, 128, 1, 16, ctypes.byref(n)) == 0 and n.value == 0
+    assert lib.qie_attention_paged_workspace(4, 1, 4, 1, 128, 4096, 16, ctypes.byref(n)) == 0 and n.value > 0
+    assert lib.qie_attention_paged_workspace(4, 1, 4, 1, 128, 4096, 16, None) == -1
