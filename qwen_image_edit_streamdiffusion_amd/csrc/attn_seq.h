@@ -74,6 +74,14 @@ __device__ __forceinline__ void seq_span(const SeqArgs& a, int b, int& start, in
 template <bool PAGED, int BM>
 __device__ __forceinline__ bool find_item(const SeqArgs& a, int idx, Item& it) {
   const int lane = threadIdx.x & 63;
+  if (!a.cu && !a.ct && a.G <= BM) {  // one token each, whole: item b is sequence b
+    if (idx >= a.B) return false;
+    it.b = idx;
+    seq_span<PAGED>(a, idx, it.start, it.n, it.kv);
+    it.blk = it.ch = 0;
+    it.nch = 1;
+    return it.n > 0;
+  }
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     int start = 0, n = 0, kv = 0, cnt = 0;
     if (b0 + lane < a.B) {
@@ -106,6 +114,20 @@ __device__ __forceinline__ bool find_item(const SeqArgs& a, int idx, Item& it) {
   return false;
 }
 
+// max / sum over the four lanes that hold a row (lanes l, l ^ 16, l ^ 32, l ^ 48) without LDS
+__device__ __forceinline__ float quad_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
 // bf16 pairs with an infinity or NaN among them
 __device__ __forceinline__ bool nonfinite(const u32x4_t w) {
   const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
@@ -136,3 +158,5 @@ __device__ __forceinline__ float special(uint32_t w, int high, bool see) {
 // attn_seq_pp.hip: blocks of kPPRows rows
 constexpr int kPPRows = 256;
 int qie_launch_seq_pp(const SeqArgs& a, bool paged, hipStream_t s);
+// attn_seq_few.hip: blocks of a.bm = 16 or 32 rows, keys shared by 4 or 8 waves
+int qie_launch_seq_few(const SeqArgs& a, bool paged, int waves, hipStream_t s);

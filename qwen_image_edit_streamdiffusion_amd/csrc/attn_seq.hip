@@ -15,13 +15,15 @@
 //   rescale only when a max grows by more than 2^8), P rounded to bf16 for the second product
 //   O^T += V^T P^T (V^T by ds_read_b64_tr_b16; the S^T registers are the P^T operand)
 // Rows past a tile's last key come from the buffer's range check as zeros.
+#include <cmath>
+
 #include "attn_seq.h"
 
 namespace {
 
 constexpr int kBM = 64;  // rows of a work-group
 
-template <bool PAGED, int NK>  // NK 32-wide steps of the head: head_dim <= 32 NK
+template <int NK>  // NK 32-wide steps of the head: head_dim <= 32 NK
 __global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
   constexpr int ND = 2 * NK;  // 16-wide blocks of the output
   __shared__ __attribute__((aligned(16))) char smem_raw[4 * kTile];  // K0 V0 K1 V1
@@ -29,7 +31,7 @@ __global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
 
   const int hk = blockIdx.x % a.Hk;
   Item it;
-  if (!find_item<PAGED, kBM>(a, blockIdx.x / a.Hk, it)) return;
+  if (!find_item<false, kBM>(a, blockIdx.x / a.Hk, it)) return;
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
   const int g = lane >> 4, ql = lane & 15;
   const int rows = it.n * a.G;
@@ -41,11 +43,7 @@ __global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
   const int lim0 = uni(lim);
   const int last = (min(rows, (it.blk + 1) * kBM) - 1) / a.G;
   const int most = a.causal ? min(it.kv, max(off + last + 1, 0)) : it.kv;
-  const int ntot = (most + kKB - 1) / kKB;
-  const int t0 = a.ct ? it.ch * a.ct : 0;
-  const int t1 = a.ct ? min(ntot, t0 + a.ct) : ntot;
-  const bool whole = !a.ct || ntot <= a.ct;
-  if (t0 > 0 && t0 >= ntot) return;  // a causal block that ends before this chunk
+  const int t1 = (most + kKB - 1) / kKB;
 
   bf16x8_t qf[NK];
   const bf16_t* qr = a.q + (int64_t)(it.start + tok) * a.ldq + (int64_t)head * a.hsq;
@@ -58,22 +56,14 @@ __global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
   // ---- tiles by LDS-DMA: a piece is 4 rows; wave w takes pieces w, w + 4, ... of K and of V. The
   // source chunk carries the XOR swizzle: K by the row, V by the row's low three bits, doubled
   const int prow = lane >> 4, pch = lane & 15;
-  const int* table = PAGED ? a.table + (int64_t)it.b * a.ldt : nullptr;
   auto dma = [&](int t, int buf) {
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       const int r0 = (wave + 4 * p) * 4;
       const int key = t * kKB + r0;
       const int nrow = min(4, it.kv - key);
-      int64_t at;
-      bool ok = nrow > 0;
-      if constexpr (PAGED) {
-        const int id = ok ? table[key >> a.pshift] : 0;
-        ok = ok && id >= 0 && id < a.pages;
-        at = (int64_t)(ok ? id : 0) * a.ps + (int64_t)hk * a.hsk + (int64_t)(key & ((1 << a.pshift) - 1)) * a.ldk;
-      } else {
-        at = ok ? (int64_t)(it.start + key) * a.ldk + (int64_t)hk * a.hsk : 0;
-      }
+      const bool ok = nrow > 0;
+      const int64_t at = ok ? (int64_t)(it.start + key) * a.ldk + (int64_t)hk * a.hsk : 0;
       const int bytes = ok ? (int)((nrow - 1) * a.ldk * 2) + a.Dh * 2 : 0;
       const uint32_t ro = prow * (uint32_t)(a.ldk * 2);
       const int row = r0 + prow;
@@ -89,9 +79,9 @@ __global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
   float m_run = kLow, l_run = 0.f;
 
   __builtin_amdgcn_s_waitcnt(0);  // q has landed: from here on the counter is the tiles'
-  if (t0 < t1) dma(t0, 0);
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
+  if (t1 > 0) dma(0, 0);
+  for (int t = 0; t < t1; ++t) {
+    const int buf = t & 1;
     if (t + 1 < t1) {
       dma(t + 1, buf ^ 1);
       asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
@@ -124,8 +114,7 @@ __global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
     for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[kb][i]);
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    mx = quad_max(mx);
     if (__any((mx - m_run) * a.c > kRescale)) {
       const float m_new = fmaxf(m_run, mx);
       const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * a.c);
@@ -191,19 +180,8 @@ __global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   }
 
-  float l = l_run + __shfl_xor(l_run, 16, 64);
-  l += __shfl_xor(l, 32, 64);
+  const float l = quad_sum(l_run);
   if (r >= rows) return;
-  if (!whole) {
-    const int64_t pi = ((int64_t)(it.start + tok) * a.H + head) * a.maxch + it.ch;
-    float* po = a.ws + pi * a.Dh;
-    float* pml = a.ws + (int64_t)a.T * a.H * a.maxch * a.Dh + pi * 2;
-#pragma unroll
-    for (int db = 0; db < ND; ++db)
-      if (16 * db + 4 * g < a.Dh) *(f32x4_t*)(po + 16 * db + 4 * g) = o[db];
-    if (g == 0) *(f32x2_t*)pml = f32x2_t{m_run, l};
-    return;
-  }
   const float inv = l == 0.f ? 0.f : 1.0f / l;  // no key seen: o is 0 as well
   bf16_t* dst = a.out + (int64_t)(it.start + tok) * a.ldo + (int64_t)head * a.hso;
 #pragma unroll
@@ -215,7 +193,6 @@ __global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
 
 // Joins the chunks of a row: o = sum_c w_c o_c / sum_c w_c l_c, w_c = exp2((m_c - max m) c). One wave a
 // (token, head); the rows that one chunk held are written already.
-template <bool PAGED>
 __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + uni(threadIdx.x >> 6);
@@ -225,7 +202,7 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
   int b = -1, start = 0, n = 0, kv = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     int s0 = 0, n0 = 0, k0 = 0;
-    if (b0 + lane < a.B) seq_span<PAGED>(a, b0 + lane, s0, n0, k0);
+    if (b0 + lane < a.B) seq_span<true>(a, b0 + lane, s0, n0, k0);
     const unsigned long long hit = __ballot(b0 + lane < a.B && s0 <= token && token < s0 + n0);
     if (hit) {
       const int l = __builtin_ctzll(hit);
@@ -246,59 +223,111 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
   const float* pml = a.ws + (int64_t)a.T * a.H * a.maxch * a.Dh + row * a.maxch * 2;
   const float* po = a.ws + row * a.maxch * a.Dh;
   float mx = kLow;
-  for (int c = 0; c < nch; ++c) mx = fmaxf(mx, pml[2 * c]);
+  for (int c = lane; c < nch; c += 64) mx = fmaxf(mx, pml[2 * c]);
+  mx = wave_max(mx);
   float l = 0.f, o0 = 0.f, o1 = 0.f;
   const int d = 2 * lane;
-  for (int c = 0; c < nch; ++c) {
-    const float w = __builtin_amdgcn_exp2f((pml[2 * c] - mx) * a.c);
-    l = __builtin_fmaf(w, pml[2 * c + 1], l);
-    if (d < a.Dh) {
-      const f32x2_t v = *(const f32x2_t*)(po + (int64_t)c * a.Dh + d);
-      o0 = __builtin_fmaf(w, v[0], o0);
-      o1 = __builtin_fmaf(w, v[1], o1);
+  for (int c0 = 0; c0 < nch; c0 += 64) {  // a lane weighs a chunk, then all lanes add 64 chunks' rows
+    float w = 0.f;
+    if (c0 + lane < nch) {
+      const f32x2_t q = *(const f32x2_t*)(pml + 2 * (c0 + lane));
+      w = __builtin_amdgcn_exp2f((q[0] - mx) * a.c);
+      l = __builtin_fmaf(w, q[1], l);
+    }
+    const int n64 = min(64, nch - c0);
+    const float* pc = po + (int64_t)c0 * a.Dh + (d < a.Dh ? d : 0);
+#pragma unroll 8
+    for (int c = 0; c < n64; ++c) {
+      const float wc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), c));
+      const f32x2_t v = *(const f32x2_t*)(pc + (int64_t)c * a.Dh);
+      o0 = __builtin_fmaf(wc, v[0], o0);
+      o1 = __builtin_fmaf(wc, v[1], o1);
     }
   }
+  l = wave_sum(l);
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   if (d < a.Dh) *(uint32_t*)(a.out + (int64_t)token * a.ldo + (int64_t)head * a.hso + d) = pack2(o0 * inv, o1 * inv);
 }
 
-// Which kernel, and how keys are cut: by what the host knows, the token, sequence and head counts and
-// the longest cache that a table can hold (0: packed sequences, never cut).
+// Which kernel, and how the keys are cut, by what the host knows: tokens, sequences, heads and the longest
+// cache that a table can hold (packed sequences: their mean length). Rows are those of one kv head,
+// tokens * G; times in us, bf16, head_dim 128, 28 heads over 4, the other side in brackets.
+//   few rows (attn_seq_few), while its blocks are about one work-group a CU and what they read again
+//     of the cache is little: 16-row blocks if 256 of them do (one prompt of 100 tokens 6.7 [64-row 9.2], 100 new
+//     tokens over 1200 13.0 [32-row 16.6]), four waves each up to 512 of them (one prompt of 200 tokens 8.8
+//     [11.6 with eight]); 32-row blocks for more, or where a long cache would be read again and again (2 x 16 rows
+//     over 20000 keys of 16 sequences: 104 [150])
+//   256-row blocks (attn_seq_pp) for the rest of a cache's rows (16 x 16 new tokens over 20000: 162 [194 few]), and
+//     for packed sequences that fill such blocks, 160 of them at least (16 prompts of 400: 53 [60 in 64-row blocks],
+//     4 of 400: 25 [21])
+//   64-row blocks (attn_seq) for shorter packed sequences.
 struct SeqPlan {
-  int bm, ct, maxch;
+  int bm, waves, ct, maxch;
 };
 
-SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, int64_t table_keys) {
-  const int64_t tiles = (table_keys + kKB - 1) / kKB;
-  const int64_t blocks = (int64_t)tokens * (heads / kv_heads) / kPPRows;  // full 256-row blocks a kv head
-  SeqPlan p{kBM, 0, 1};
-  const bool pp = blocks >= seqs && blocks * kv_heads >= 64;
-  if (pp) p.bm = kPPRows;
-  const int ct = table_keys == 0 ? 0 : pp ? (blocks * kv_heads < 512 ? 32 : 0) : 8;
-  if (ct && tiles > ct) {
-    p.ct = ct;
-    p.maxch = (int)((tiles + ct - 1) / ct);
+SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, bool causal, int64_t table_keys) {
+  const double rows = (double)tokens * (heads / kv_heads);
+  const double per = rows / seqs;  // rows of a sequence
+  const bool paged = table_keys > 0;
+  const double keys = paged ? (double)table_keys : (double)tokens / seqs;
+  const double g16 = kv_heads * fmax(seqs, rows / 16), g32 = kv_heads * fmax(seqs, rows / 32);
+  SeqPlan p{kBM, 8, 0, 1};
+  if (!paged) {
+    if (g16 <= 512) {
+      p.bm = 16;
+      p.waves = g16 <= 256 ? 8 : 4;
+    } else if (per >= (causal ? 1024 : 150) && kv_heads * rows / kPPRows >= 160) {
+      p.bm = kPPRows;
+    }
+    return p;
+  }
+  if (per <= 32 || (g32 <= 512 && g32 * keys <= 1.5e6)) {
+    const bool reread = per > 16 && g16 * keys > 4e5;
+    p.bm = per <= 16 || (g16 <= 512 && !reread) ? 16 : 32;
+    p.waves = per > 16 && p.bm == 16 && g16 > 256 ? 4 : 8;
+  } else {
+    p.bm = kPPRows;
+  }
+  // Cuts: work-groups that do not fill the chip share a row's keys, in chunks of ct tiles whose fp32 parts a
+  // second kernel joins. Enough chunks for 256 work-groups, no more; for few rows at least
+  // 1.4 sqrt(tiles) tiles each, where a chunk's time and the join's meet (one token over 32768 keys: 16 or
+  // 32 tiles 26.4, 8 or 64 34), and none up to 1024 keys (one launch: 10.1 [10.9]). At most 64 tiles, so that a
+  // long sequence among short ones is shared too (48 sequences of 900 .. 32768: 298 at 32 tiles, 305 at 64, 840 uncut).
+  const double tiles = (double)((table_keys + kKB - 1) / kKB);
+  const double groups = p.bm == kPPRows ? kv_heads * fmax(1.0, rows / kPPRows) : p.bm == 16 ? g16 : g32;
+  double ct = tiles * groups / 256;
+  if (p.bm == kPPRows) {
+    if (groups >= 512 || (groups >= 256 && tiles <= 128)) return p;
+    ct = fmax(ct, 8.0);
+  } else {
+    if (tiles <= 16) return p;
+    ct = fmax(fmax(ct, 1.4 * sqrt(tiles)), 8.0);
+  }
+  ct = fmin(ct, 64.0);
+  if (tiles > ct) {
+    const int n = (int)ceil(tiles / ct - 1e-9);  // chunks of one size
+    p.ct = (int)ceil(tiles / n);
+    p.maxch = (int)ceil(tiles / p.ct);
   }
   return p;
 }
 
-template <bool PAGED>
-int launch_seq(SeqArgs& a, const SeqPlan& p, hipStream_t s) {
+int launch_seq(SeqArgs& a, const SeqPlan& p, bool paged, hipStream_t s) {
   a.bm = p.bm;
   a.ct = p.ct;
   a.maxch = p.maxch;
-  if (p.bm == kPPRows) {
-    const int rc = qie_launch_seq_pp(a, PAGED, s);
+  if (p.bm != kBM) {
+    const int rc = p.bm == kPPRows ? qie_launch_seq_pp(a, paged, s) : qie_launch_seq_few(a, paged, p.waves, s);
     if (rc) return rc;
   } else {
     const int64_t rb = (int64_t)a.T * a.G / kBM + a.B;  // at least the row blocks of any lengths
-    const int64_t grid = rb * a.maxch * a.Hk;
+    const int64_t grid = rb * a.Hk;
     if (grid > INT32_MAX) return QIE_ERR_UNSUPPORTED;
-    if (a.Dh <= 64) attn_seq_kernel<PAGED, 2><<<(unsigned)grid, 256, 0, s>>>(a);
-    else if (a.Dh <= 96) attn_seq_kernel<PAGED, 3><<<(unsigned)grid, 256, 0, s>>>(a);
-    else attn_seq_kernel<PAGED, 4><<<(unsigned)grid, 256, 0, s>>>(a);
+    if (a.Dh <= 64) attn_seq_kernel<2><<<(unsigned)grid, 256, 0, s>>>(a);
+    else if (a.Dh <= 96) attn_seq_kernel<3><<<(unsigned)grid, 256, 0, s>>>(a);
+    else attn_seq_kernel<4><<<(unsigned)grid, 256, 0, s>>>(a);
   }
-  if (a.ct) attn_seq_join_kernel<PAGED><<<(unsigned)(((int64_t)a.T * a.H + 3) / 4), 256, 0, s>>>(a);
+  if (a.ct) attn_seq_join_kernel<<<(unsigned)(((int64_t)a.T * a.H + 3) / 4), 256, 0, s>>>(a);
   return qie_last_error();
 }
 
@@ -330,14 +359,14 @@ extern "C" int qie_attention_packed_bf16(const void* q, int64_t ldq, int64_t hsq
   a.B = seqs; a.T = tokens; a.H = heads; a.Hk = kv_heads; a.G = heads / kv_heads; a.Dh = head_dim;
   a.causal = causal != 0;
   a.c = scale * 1.4426950408889634f;
-  return launch_seq<false>(a, seq_plan(tokens, seqs, heads, kv_heads, 0), (hipStream_t)stream);
+  return launch_seq(a, seq_plan(tokens, seqs, heads, kv_heads, causal != 0, 0), false, (hipStream_t)stream);
 }
 
 extern "C" int qie_attention_paged_workspace(int tokens, int seqs, int heads, int kv_heads, int head_dim,
                                              int table_width, int page_size, int64_t* bytes) {
   QIE_CHECK_ARG(bytes && tokens >= 0 && seqs > 0 && heads > 0 && kv_heads > 0 && head_dim > 0 && table_width > 0 &&
                 page_size > 0 && (int64_t)table_width * page_size <= INT32_MAX / 2);
-  const SeqPlan p = seq_plan(tokens, seqs, heads, kv_heads, (int64_t)table_width * page_size);
+  const SeqPlan p = seq_plan(tokens, seqs, heads, kv_heads, true, (int64_t)table_width * page_size);
   *bytes = p.ct ? (int64_t)tokens * heads * p.maxch * (head_dim + 2) * 4 : 0;
   return QIE_OK;
 }
@@ -372,6 +401,6 @@ extern "C" int qie_attention_paged_bf16(const void* q, int64_t ldq, int64_t hsq,
   a.kv_lens = kv_lens;
   a.width = table_width; a.pages = num_pages; a.pshift = __builtin_ctz(page_size);
   a.ws = (float*)workspace;
-  return launch_seq<true>(a, seq_plan(tokens, seqs, heads, kv_heads, (int64_t)table_width * page_size),
-                          (hipStream_t)stream);
+  return launch_seq(a, seq_plan(tokens, seqs, heads, kv_heads, true, (int64_t)table_width * page_size), true,
+                    (hipStream_t)stream);
 }

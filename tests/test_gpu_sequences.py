@@ -561,7 +561,7 @@ def test_refusals():
             lambda: ops.attention_packed(q, k, k, cu, out=z(4, 4, 32)),
             lambda: ops.attention_packed(q, k, k, cu, out=z(1, 4, 64).expand(4, 4, 64)),
             lambda: ops.attention_packed(z(4, 4, 66)[..., 1:65], k, k, cu)]
-    q2, t, n = z(2, 4, 128), z(2, 40, dt=i32), z(2, dt=i32)
+    q2, t, n = z(2, 4, 128), z(2, 400, dt=i32), z(2, dt=i32)
     bad += [lambda: ops.attention_paged(z(3, 4, 128), kp, vp, t, n), lambda: ops.attention_paged(q2, kp, vp, t.long(), n),
             lambda: ops.attention_paged(q2, kp, vp, t, n[:1]), lambda: ops.attention_paged(q2, kp, vp, t, n, cu_seqlens=n),
             lambda: ops.attention_paged(z(2, 4, 64), kp, vp, t, n), lambda: ops.attention_paged(q2, kp, vp.float(), t, n),

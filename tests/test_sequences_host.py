@@ -81,7 +81,7 @@ def test_entry_points_refuse_on_the_host(lib):
         assert packed(**kw) == -1, kw
     assert packed(T=0) == 0
 
-    ok4 = dict(ok3, N=4, P=16, ps=2048, hsk=2048, table=16, ldt=64, W=64, kvl=16, ws=16, wsb=1 << 40)
+    ok4 = dict(ok3, N=4, P=16, ps=2048, hsk=2048, table=16, ldt=4096, W=4096, kvl=16, ws=16, wsb=1 << 40)
 
     def paged(**kw):
         a = {**ok4, **kw}
@@ -89,7 +89,7 @@ def test_entry_points_refuse_on_the_host(lib):
                                             a["ldk"], a["table"], a["ldt"], a["W"], a["kvl"], a["cu"], a["B"], a["T"], a["H"],
                                             a["Hk"], a["dh"], a["sc"], a["out"], a["ldo"], a["hso"], a["ws"], a["wsb"], None)
     for kw in refused + (dict(table=None), dict(kvl=None), dict(cu=None), dict(N=0), dict(P=8), dict(P=48), dict(P=2048),
-                         dict(ps=2052), dict(W=0), dict(ldt=63), dict(W=1 << 27, ldt=1 << 27), dict(ws=None), dict(wsb=64),
+                         dict(ps=2052), dict(W=0), dict(ldt=4095), dict(W=1 << 27, ldt=1 << 27), dict(ws=None), dict(wsb=64),
                          dict(ws=20)):
         assert paged(**kw) == -1, kw
     n = ctypes.c_int64(-1)
