@@ -433,7 +433,9 @@ int qie_attention_packed_bf16(const void* q, int64_t ldq, int64_t hsq, const voi
  * page page_table[b][j / page_size] (a page outside the pool reads as zeros), pages as in
  * qie_rope_append_bf16. A row that sees no key is 0. Long rows are cut into chunks of keys whose
  * fp32 partials meet in `workspace` (>= qie_attention_paged_workspace bytes, 16-byte aligned, not
- * shared with a call that may run at the same time); the cuts go by a row's own sequence only. */
+ * shared with a call that may run at the same time; 0 bytes, and NULL is fine, for tables of up to
+ * 1024 tokens). The cuts go by the call's counts, never by the values of lengths or tables: in calls
+ * of one shape a row's bits do not depend on the other sequences. */
 int qie_attention_paged_workspace(int tokens, int seqs, int heads, int kv_heads, int head_dim, int table_width,
                                   int page_size, int64_t* bytes);
 int qie_attention_paged_bf16(const void* q, int64_t ldq, int64_t hsq, const void* k_pages, const void* v_pages,

@@ -70,6 +70,17 @@ __device__ __forceinline__ void seq_span(const SeqArgs& a, int b, int& start, in
   kv = PAGED ? min(max(a.kv_lens[b], 0), a.width << a.pshift) : n;
 }
 
+// inclusive sum over the lanes: within rows of 16, then a row's last lane to the next row, then 31 to 32 ..
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
 // The idx-th (row block, key chunk) over all sequences: a wave-wide scan of the sequences' counts.
 template <bool PAGED, int BM>
 __device__ __forceinline__ bool find_item(const SeqArgs& a, int idx, Item& it) {
@@ -89,27 +100,22 @@ __device__ __forceinline__ bool find_item(const SeqArgs& a, int idx, Item& it) {
       cnt = (n * a.G + BM - 1) / BM;
       if (a.ct) cnt *= max(1, (kv + a.ct * kKB - 1) / (a.ct * kKB));
     }
-    int pre = cnt;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(pre, o, 64);
-      if (lane >= o) pre += u;
-    }
+    const int pre = wave_scan(cnt);
     const unsigned long long hit = __ballot(pre > idx);
     if (hit) {
       const int l = __builtin_ctzll(hit);
-      it.b = uni(b0 + l);
-      it.start = uni(__shfl(start, l, 64));
-      it.n = uni(__shfl(n, l, 64));
-      it.kv = uni(__shfl(kv, l, 64));
-      const int j = idx - uni(__shfl(pre - cnt, l, 64));
+      it.b = b0 + l;
+      it.start = __builtin_amdgcn_readlane(start, l);
+      it.n = __builtin_amdgcn_readlane(n, l);
+      it.kv = __builtin_amdgcn_readlane(kv, l);
+      const int j = idx - __builtin_amdgcn_readlane(pre - cnt, l);
       it.nch = a.ct ? max(1, (it.kv + a.ct * kKB - 1) / (a.ct * kKB)) : 1;
       const int nblk = (it.n * a.G + BM - 1) / BM;
       it.ch = j / nblk;               // neighbours read the same keys
       it.blk = nblk - 1 - j % nblk;  // the longest rows of a causal sequence first
       return true;
     }
-    idx -= uni(__shfl(pre, 63, 64));
+    idx -= __builtin_amdgcn_readlane(pre, 63);
   }
   return false;
 }

@@ -8,10 +8,11 @@
 // head hk G + r % G. K and V are then read once for G heads, a single token still fills G rows of a
 // matrix instruction, and a causal diagonal is G times narrower in rows.
 //
-// attn_seq_kernel: one work-group = 4 waves = 64 rows of one (sequence, kv head), 64-key tiles,
-// double-buffered in LDS by buffer_load ... lds. Per wave and tile, 16 rows:
+// attn_seq_kernel: one work-group = 4 waves = 64 rows of one (sequence, kv head), 32-key tiles,
+// double-buffered in LDS by buffer_load ... lds (32 KiB, four work-groups a CU: short sequences are
+// bound by the latency of a chain of loads, which other work-groups fill). Per wave and tile, 16 rows:
 //   S^T = K Q^T (mfma 16x16x32, K rows by ds_read_b128 from an XOR-swizzled image, Q^T in registers)
-//   a lane holds 16 keys of one row: online softmax in log2 units (running max and sum in fp32, the
+//   a lane holds 8 keys of one row: online softmax in log2 units (running max and sum in fp32, the
 //   rescale only when a max grows by more than 2^8), P rounded to bf16 for the second product
 //   O^T += V^T P^T (V^T by ds_read_b64_tr_b16; the S^T registers are the P^T operand)
 // Rows past a tile's last key come from the buffer's range check as zeros.
@@ -23,28 +24,87 @@ namespace {
 
 constexpr int kBM = 64;  // rows of a work-group
 
-template <int NK>  // NK 32-wide steps of the head: head_dim <= 32 NK
-__global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
-  constexpr int ND = 2 * NK;  // 16-wide blocks of the output
-  __shared__ __attribute__((aligned(16))) char smem_raw[4 * kTile];  // K0 V0 K1 V1
+template <bool PAGED, int NK>  // NK 32-wide steps of the head: head_dim <= 32 NK
+__global__ void __launch_bounds__(256, NK == 4 ? 3 : 4) attn_seq_kernel(SeqArgs a) {
+  constexpr int ND = 2 * NK;     // 16-wide blocks of the output
+  constexpr int KT = 32, KB = KT / 16, NP = KT / 16;  // keys of a tile, their blocks, pieces of a wave
+  constexpr int TILE = KT * kRowB;
+  __shared__ __attribute__((aligned(16))) char smem_raw[4 * TILE];  // K0 V0 K1 V1
   char QIE_LDS* smem = (char QIE_LDS*)smem_raw;
 
   const int hk = blockIdx.x % a.Hk;
   Item it;
-  if (!find_item<false, kBM>(a, blockIdx.x / a.Hk, it)) return;
+  if (!find_item<PAGED, kBM>(a, blockIdx.x / a.Hk, it)) return;
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
   const int g = lane >> 4, ql = lane & 15;
   const int rows = it.n * a.G;
+  const int last = (min(rows, (it.blk + 1) * kBM) - 1) / a.G;
+  const int off = it.kv - it.n;
+  const int most = a.causal ? min(it.kv, max(off + last + 1, 0)) : it.kv;
+  const int ntot = (most + kKB - 1) / kKB;  // in the 64-key units that chunks are counted in
+  const int t0 = PAGED && a.ct ? it.ch * a.ct * 2 : 0;
+  const int t1 = min((most + KT - 1) / KT, PAGED && a.ct ? t0 + 2 * a.ct : INT32_MAX);
+  const bool whole = !PAGED || !a.ct || ntot <= a.ct;
+  if (t0 > 0 && t0 >= t1) return;  // a causal block that ends before this chunk
+
+  // ---- tiles by LDS-DMA: a piece is 4 rows; wave w takes pieces w, w + 4, ... of K and of V. The
+  // source chunk carries the XOR swizzle: K by the row, V by the row's low three bits, doubled
+  const uint32_t ldb = (uint32_t)(a.ldk * 2);
+  uint32_t ko[NP], vo[NP];
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    const int row = (wave + 4 * p) * 4 + g, ck = ql ^ (row & 15), cv = ql ^ ((row & 7) << 1);
+    const uint32_t ro = (PAGED ? row & 15 : row) * ldb;  // pages: within the 16-row half that piece p lies in
+    ko[p] = ck * 8 < a.Dh ? ro + ck * 16 : 0x80000000u;
+    vo[p] = cv * 8 < a.Dh ? ro + cv * 16 : 0x80000000u;
+  }
+  const int64_t at0 = (int64_t)hk * a.hsk + (PAGED ? 0 : (int64_t)it.start * a.ldk);
+  const int* table = PAGED ? a.table + (int64_t)it.b * a.ldt : nullptr;
+  int tb = t0, pg[NP] = {};  // lane i: the pages of tile tb + i's halves (-1: outside the pool)
+  auto pages = [&](int from) {
+    tb = from;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int64_t page = ((int64_t)(from + lane) * KT + 16 * p) >> a.pshift;
+      int id = -1;
+      if (page < a.width) id = table[page];
+      pg[p] = id >= 0 && id < a.pages ? id : -1;
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+  };
+  auto dma = [&](int t, int st) {
+    i32x4_t kr, vr;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      if constexpr (PAGED) {
+        const int key = t * KT + 16 * p, nrow = min(16, it.kv - key);
+        const int id = __builtin_amdgcn_readlane(pg[p], t - tb);
+        const bool ok = nrow > 0 && id >= 0;
+        const int64_t at = at0 + (ok ? (int64_t)id * a.ps + (int64_t)(key & ((1 << a.pshift) - 1)) * a.ldk : 0);
+        const int bytes = ok ? (nrow - 1) * (int)ldb + a.Dh * 2 : 0;
+        kr = seq_rsrc(a.k + at, bytes);
+        vr = seq_rsrc(a.v + at, bytes);
+      } else if (p == 0) {
+        const int64_t at = at0 + (int64_t)t * KT * a.ldk;
+        const int bytes = (min(KT, it.kv - t * KT) - 1) * (int)ldb + a.Dh * 2;  // zeros past the sequence
+        kr = seq_rsrc(a.k + at, bytes);
+        vr = seq_rsrc(a.v + at, bytes);
+      }
+      const int r0 = (wave + 4 * p) * 4;
+      seq_dma(kr, smem + (2 * st) * TILE + r0 * kRowB, ko[p]);
+      seq_dma(vr, smem + (2 * st + 1) * TILE + r0 * kRowB, vo[p]);
+    }
+  };
+  if (t0 < t1) {
+    if constexpr (PAGED) pages(t0);
+    dma(t0, 0);
+    if (t0 + 1 < t1) dma(t0 + 1, 1);
+  }
+
   const int r = it.blk * kBM + wave * 16 + ql;
   const int tok = min(r, rows - 1) / a.G, head = hk * a.G + min(r, rows - 1) % a.G;
-  // keys that a row sees; of the wave's first row and of the block's last one
-  const int off = it.kv - it.n;
-  const int lim = a.causal ? min(it.kv, max(off + tok + 1, 0)) : it.kv;
-  const int lim0 = uni(lim);
-  const int last = (min(rows, (it.blk + 1) * kBM) - 1) / a.G;
-  const int most = a.causal ? min(it.kv, max(off + last + 1, 0)) : it.kv;
-  const int t1 = (most + kKB - 1) / kKB;
-
+  const int lim = a.causal ? min(it.kv, max(off + tok + 1, 0)) : it.kv;  // keys that this row sees
+  const int lim0 = uni(lim);                                             // fewest of the wave
   bf16x8_t qf[NK];
   const bf16_t* qr = a.q + (int64_t)(it.start + tok) * a.ldq + (int64_t)head * a.hsq;
 #pragma unroll
@@ -52,47 +112,19 @@ __global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
     qf[ks] = bf16x8_t{};
     if (32 * ks + 8 * g < a.Dh) qf[ks] = *(const bf16x8_t*)(qr + 32 * ks + 8 * g);
   }
-
-  // ---- tiles by LDS-DMA: a piece is 4 rows; wave w takes pieces w, w + 4, ... of K and of V. The
-  // source chunk carries the XOR swizzle: K by the row, V by the row's low three bits, doubled
-  const int prow = lane >> 4, pch = lane & 15;
-  auto dma = [&](int t, int buf) {
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const int r0 = (wave + 4 * p) * 4;
-      const int key = t * kKB + r0;
-      const int nrow = min(4, it.kv - key);
-      const bool ok = nrow > 0;
-      const int64_t at = ok ? (int64_t)(it.start + key) * a.ldk + (int64_t)hk * a.hsk : 0;
-      const int bytes = ok ? (int)((nrow - 1) * a.ldk * 2) + a.Dh * 2 : 0;
-      const uint32_t ro = prow * (uint32_t)(a.ldk * 2);
-      const int row = r0 + prow;
-      const int ck = pch ^ (row & 15), cv = pch ^ ((row & 7) << 1);
-      seq_dma(seq_rsrc(a.k + at, bytes), smem + (2 * buf) * kTile + r0 * kRowB, ck * 8 < a.Dh ? ro + ck * 16 : 0x80000000u);
-      seq_dma(seq_rsrc(a.v + at, bytes), smem + (2 * buf + 1) * kTile + r0 * kRowB, cv * 8 < a.Dh ? ro + cv * 16 : 0x80000000u);
-    }
-  };
-
   f32x4_t o[ND];
 #pragma unroll
   for (int db = 0; db < ND; ++db) o[db] = f32x4_t{};
   float m_run = kLow, l_run = 0.f;
 
-  __builtin_amdgcn_s_waitcnt(0);  // q has landed: from here on the counter is the tiles'
-  if (t1 > 0) dma(0, 0);
-  for (int t = 0; t < t1; ++t) {
-    const int buf = t & 1;
-    if (t + 1 < t1) {
-      dma(t + 1, buf ^ 1);
-      asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    }
-    const char QIE_LDS* kt = smem + (2 * buf) * kTile;
-    const char QIE_LDS* vt = kt + kTile;
-    f32x4_t s[4];
+  __builtin_amdgcn_s_waitcnt(0);  // q and two tiles: from here on the counter is the tiles'
+  asm volatile("s_barrier" ::: "memory");
+  for (int t = t0; t < t1; ++t) {
+    const char QIE_LDS* kt = smem + (2 * (t & 1)) * TILE;  // t0 is even
+    const char QIE_LDS* vt = kt + TILE;
+    f32x4_t s[KB];
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb) {
+    for (int kb = 0; kb < KB; ++kb) {
       s[kb] = f32x4_t{};
 #pragma unroll
       for (int ks = 0; ks < NK; ++ks) {
@@ -100,18 +132,18 @@ __global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
         s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, qf[ks], s[kb], 0, 0, 0);
       }
     }
-    const int kv0 = t * kKB;
-    const bool masked = kv0 + kKB > lim0;
+    const int kv0 = t * KT;
+    const bool masked = kv0 + KT > lim0;
     if (masked) {
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (kv0 + kb * 16 + 4 * g + i >= lim) s[kb][i] = -INFINITY;
     }
     float mx = s[0][0];
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[kb][i]);
     mx = quad_max(mx);
@@ -124,18 +156,18 @@ __global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
       for (int db = 0; db < ND; ++db) o[db] *= alpha;
     }
     const float mc = m_run * a.c;
-    bf16x8_t pf[2];
+    bf16x8_t pf;
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], a.c, -mc));
         l_run += p;
-        pf[kb >> 1][4 * (kb & 1) + i] = (__bf16)p;
+        pf[4 * kb + i] = (__bf16)p;
       }
-    // V^T fragment: lane's d = 16 db + ql, keys 32 k2 + 4 g + 0..3 and 16 further
-    auto vfrag = [&](int k2, int db) -> bf16x8_t {
-      const int row = 32 * k2 + 4 * g + (ql >> 2);
+    // V^T fragment: lane's d = 16 db + ql, keys 4 g + 0..3 and 16 further
+    auto vfrag = [&](int db) -> bf16x8_t {
+      const int row = 4 * g + (ql >> 2);
       const int ch = (2 * db + ((ql & 3) >> 1)) ^ ((row & 7) << 1);
       const char QIE_LDS* p0 = vt + row * kRowB + (ch << 4) + 8 * (ql & 1);
       const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t QIE_LDS*)p0);
@@ -146,20 +178,18 @@ __global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
     bool bad = false;
     if (masked) {
 #pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2)
-#pragma unroll
-        for (int db = 0; db < ND; ++db) bad |= nonfinite(__builtin_bit_cast(u32x4_t, vfrag(k2, db)));
-      asm volatile("" ::: "memory");  // read again below: keeping all of them costs 64 registers
+      for (int db = 0; db < ND; ++db) bad |= nonfinite(__builtin_bit_cast(u32x4_t, vfrag(db)));
+      asm volatile("" ::: "memory");  // read again below: keeping all of them costs registers
     }
     if (__builtin_expect(__any(bad), 0)) {
       // the finite values as ever, then what a row sees of the others
 #pragma unroll
-      for (int j = 0; j < 2 * ND; ++j) {
+      for (int db = 0; db < ND; ++db) {
         asm volatile("" ::: "memory");
-        o[j % ND] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(finite(vfrag(j / ND, j % ND)), pf[j / ND], o[j % ND], 0, 0, 0);
+        o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(finite(vfrag(db)), pf, o[db], 0, 0, 0);
       }
 #pragma unroll 1
-      for (int j = 0; j < kKB; ++j) {
+      for (int j = 0; j < KT; ++j) {
         const char QIE_LDS* vr = vt + j * kRowB + 8 * (g & 1);
         const bool see = kv0 + j < lim;
 #pragma unroll
@@ -171,18 +201,32 @@ __global__ void __launch_bounds__(256) attn_seq_kernel(SeqArgs a) {
       }
     } else {
 #pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2)
-#pragma unroll
-        for (int db = 0; db < ND; ++db)
-          o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vfrag(k2, db), pf[k2], o[db], 0, 0, 0);
+      for (int db = 0; db < ND; ++db) o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vfrag(db), pf, o[db], 0, 0, 0);
     }
-    // this tile's reads are done: its buffer is free for the one after the next
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (t + 1 == t1) break;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // this tile's stage is free
+    if (t + 2 < t1) {
+      if constexpr (PAGED)
+        if (t + 2 - tb >= 64) pages(t + 2);
+      dma(t + 2, t & 1);
+      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * NP) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    }
   }
 
   const float l = quad_sum(l_run);
   if (r >= rows) return;
-  const float inv = l == 0.f ? 0.f : 1.0f / l;  // no key seen: o is 0 as well
+  if (!whole) {
+    const int64_t pi = ((int64_t)(it.start + tok) * a.H + head) * a.maxch + it.ch;
+    float* po = a.ws + pi * a.Dh;
+#pragma unroll
+    for (int db = 0; db < ND; ++db)
+      if (16 * db + 4 * g < a.Dh) *(f32x4_t*)(po + 16 * db + 4 * g) = o[db];
+    if (g == 0) *(f32x2_t*)(a.ws + (int64_t)a.T * a.H * a.maxch * a.Dh + pi * 2) = f32x2_t{m_run, l};
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
   bf16_t* dst = a.out + (int64_t)(it.start + tok) * a.ldo + (int64_t)head * a.hso;
 #pragma unroll
   for (int db = 0; db < ND; ++db)
@@ -249,67 +293,81 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
   if (d < a.Dh) *(uint32_t*)(a.out + (int64_t)token * a.ldo + (int64_t)head * a.hso + d) = pack2(o0 * inv, o1 * inv);
 }
 
-// Which kernel, and how the keys are cut, by what the host knows: tokens, sequences, heads and the longest
-// cache that a table can hold (packed sequences: their mean length). Rows are those of one kv head,
-// tokens * G; times in us, bf16, head_dim 128, 28 heads over 4, the other side in brackets.
-//   few rows (attn_seq_few), while its blocks are about one work-group a CU and what they read again
-//     of the cache is little: 16-row blocks if 256 of them do (one prompt of 100 tokens 6.7 [64-row 9.2], 100 new
-//     tokens over 1200 13.0 [32-row 16.6]), four waves each up to 512 of them (one prompt of 200 tokens 8.8
-//     [11.6 with eight]); 32-row blocks for more, or where a long cache would be read again and again (2 x 16 rows
-//     over 20000 keys of 16 sequences: 104 [150])
-//   256-row blocks (attn_seq_pp) for the rest of a cache's rows (16 x 16 new tokens over 20000: 162 [194 few]), and
-//     for packed sequences that fill such blocks, 160 of them at least (16 prompts of 400: 53 [60 in 64-row blocks],
-//     4 of 400: 25 [21])
-//   64-row blocks (attn_seq) for shorter packed sequences.
+// Which kernel, and how the keys are cut, by what the host knows: tokens, sequences, heads and the
+// longest cache that a table can hold (packed sequences: their mean length). Rows are those of one kv
+// head, tokens * G; a group is a (row block, kv head). Times in us, bf16, head_dim 128, 28 heads over 4
+// unless said, the other side in brackets.
+//   few rows (attn_seq_few), 16-row blocks: up to 256 groups with eight waves each (one prompt of 100
+//     tokens 6.6 [9.2 in 64-row blocks]), up to 512 with four, two a CU (one prompt of 200: 8.4 [11.6 with
+//     eight]). 32-row blocks where 16-row ones would be more, or read a long cache again and again (4 new
+//     tokens over 20000 keys of 16 sequences: 104 [150]).
+//   64-row blocks (attn_seq): shorter packed sequences (16 prompts of 400: 42 [52 in 256-row blocks]), a short
+//     cache's many rows (16 x 100 new tokens over 300: 20 [25]), and 33 .. 64 rows of a sequence over a long one (16 x
+//     8 new tokens over 20000: 107 [156 in 32-row blocks]).
+//   256-row blocks (attn_seq_pp) where there are about 200 of them: packed sequences of 700 tokens in the
+//     mean (1500 where causal heads share nothing and a block spans 256 tokens: 64 sequences of 1000, 24 heads over 24,
+//     687 [597 in 64-row blocks]; of 28 over 4: 551 [598]), long caches (16 x 100 new tokens over 5000: 144 [179]).
 struct SeqPlan {
   int bm, waves, ct, maxch;
 };
 
 SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, bool causal, int64_t table_keys) {
-  const double rows = (double)tokens * (heads / kv_heads);
-  const double per = rows / seqs;  // rows of a sequence
   const bool paged = table_keys > 0;
+  const double rows = (double)tokens * (heads / kv_heads), per = rows / seqs;  // in all, of a sequence
   const double keys = paged ? (double)table_keys : (double)tokens / seqs;
-  const double g16 = kv_heads * fmax(seqs, rows / 16), g32 = kv_heads * fmax(seqs, rows / 32);
-  SeqPlan p{kBM, 8, 0, 1};
+  const double g16 = kv_heads * fmax(seqs, rows / 16), g32 = kv_heads * fmax(seqs, rows / 32),
+               g64 = kv_heads * fmax(seqs, rows / kBM), g256 = kv_heads * fmax(1.0, rows / kPPRows);
+  const int few16 = g16 <= 256 ? 8 : 4;
+  SeqPlan p{kBM, few16, 0, 1};
   if (!paged) {
-    if (g16 <= 512) {
-      p.bm = 16;
-      p.waves = g16 <= 256 ? 8 : 4;
-    } else if (per >= (causal ? 1024 : 150) && kv_heads * rows / kPPRows >= 160) {
-      p.bm = kPPRows;
-    }
+    if (g16 <= 512) p.bm = 16;
+    else if (keys >= (causal && heads == kv_heads ? 1500 : 700) && g256 >= 200) p.bm = kPPRows;
     return p;
   }
-  if (per <= 32 || (g32 <= 512 && g32 * keys <= 1.5e6)) {
-    const bool reread = per > 16 && g16 * keys > 4e5;
-    p.bm = per <= 16 || (g16 <= 512 && !reread) ? 16 : 32;
-    p.waves = per > 16 && p.bm == 16 && g16 > 256 ? 4 : 8;
+  if (per <= 16) {
+    p.bm = 16;
+    p.waves = 8;
+  } else if (keys <= 512) {
+    p.bm = g16 <= 512 ? 16 : kBM;
+  } else if (per > 32 && per <= 64 && g32 * keys > 3e5) {
+    p.bm = kBM;
+  } else if (per <= 32 || (g32 <= 512 && g32 * keys <= 1.5e6)) {
+    p.bm = g16 <= 512 && g16 * keys <= 4e5 ? 16 : 32;
+    if (p.bm == 32) p.waves = 8;
   } else {
-    p.bm = kPPRows;
+    p.bm = keys <= 2048 && g256 < 200 ? kBM : kPPRows;
   }
-  // Cuts: work-groups that do not fill the chip share a row's keys, in chunks of ct tiles whose fp32 parts a
-  // second kernel joins. Enough chunks for 256 work-groups, no more; for few rows at least
-  // 1.4 sqrt(tiles) tiles each, where a chunk's time and the join's meet (one token over 32768 keys: 16 or
-  // 32 tiles 26.4, 8 or 64 34), and none up to 1024 keys (one launch: 10.1 [10.9]). At most 64 tiles, so that a
-  // long sequence among short ones is shared too (48 sequences of 900 .. 32768: 298 at 32 tiles, 305 at 64, 840 uncut).
+  // Cuts: groups that do not fill the chip share a row's keys, in chunks whose fp32 parts a second kernel
+  // joins: as many as fit 256 CUs at once (1000 new tokens over 5000 keys, two of 40 tiles: 99 [uncut 138, three
+  // chunks 124]; three 64-row work-groups fit a CU), of 8 tiles at least. Up to 1024 keys, none (one
+  // token: 10.1 in one launch [10.9 in two]). Few rows: 1.4 sqrt(tiles) tiles at least, where a chunk's time
+  // and the join's meet (one token over 32768 keys: 26.4 with 16 or 32 tiles [34 with 8 or 64]). Long tables are
+  // cut all the same, so that a long sequence among short ones is shared (48 tokens over 900 .. 32768 keys:
+  // 298 [840 uncut]): into 32 tiles (4 and 16 new tokens over 20000 keys of 16 sequences: 104 and 167 [132 and 240
+  // with 64]), 64 where there is one sequence or the groups fill the chip without a cut.
   const double tiles = (double)((table_keys + kKB - 1) / kKB);
-  const double groups = p.bm == kPPRows ? kv_heads * fmax(1.0, rows / kPPRows) : p.bm == 16 ? g16 : g32;
-  double ct = tiles * groups / 256;
-  if (p.bm == kPPRows) {
-    if (groups >= 512 || (groups >= 256 && tiles <= 128)) return p;
-    ct = fmax(ct, 8.0);
-  } else {
-    if (tiles <= 16) return p;
-    ct = fmax(fmax(ct, 1.4 * sqrt(tiles)), 8.0);
-  }
-  ct = fmin(ct, 64.0);
+  if (tiles <= 16 || (p.bm == kBM && tiles <= 32)) return p;
+  const double half = per > 16 ? 0.5 * seqs * kv_heads : 0;  // sequences end inside a block
+  const double groups = p.bm == 16 ? g16 + half : p.bm == 32 ? g32 + half : p.bm == kBM ? g64 / 3 : g256 + half;
+  if (p.bm == kPPRows && groups >= 512) return p;
+  double n = fmax(1.0, floor(256 / groups));
+  if (n == 1 && 2 * groups <= 290) n = 2;
+  const double low = p.bm < kBM ? fmax(8.0, 1.4 * sqrt(tiles)) : 8;
+  double ct = fmax(tiles / n, low);
+  if (per <= 64 || tiles > 128) ct = fmin(ct, groups >= 256 || (per > 64 && seqs == 1) ? 64 : fmax(32.0, low));
   if (tiles > ct) {
-    const int n = (int)ceil(tiles / ct - 1e-9);  // chunks of one size
-    p.ct = (int)ceil(tiles / n);
+    p.ct = (int)ceil(tiles / ceil(tiles / ct - 1e-9));  // chunks of one size
     p.maxch = (int)ceil(tiles / p.ct);
   }
   return p;
+}
+
+template <bool PAGED>
+int launch(const SeqArgs& a, unsigned grid, hipStream_t s) {
+  if (a.Dh <= 64) attn_seq_kernel<PAGED, 2><<<grid, 256, 0, s>>>(a);
+  else if (a.Dh <= 96) attn_seq_kernel<PAGED, 3><<<grid, 256, 0, s>>>(a);
+  else attn_seq_kernel<PAGED, 4><<<grid, 256, 0, s>>>(a);
+  return qie_last_error();
 }
 
 int launch_seq(SeqArgs& a, const SeqPlan& p, bool paged, hipStream_t s) {
@@ -321,11 +379,10 @@ int launch_seq(SeqArgs& a, const SeqPlan& p, bool paged, hipStream_t s) {
     if (rc) return rc;
   } else {
     const int64_t rb = (int64_t)a.T * a.G / kBM + a.B;  // at least the row blocks of any lengths
-    const int64_t grid = rb * a.Hk;
+    const int64_t grid = rb * a.maxch * a.Hk;
     if (grid > INT32_MAX) return QIE_ERR_UNSUPPORTED;
-    if (a.Dh <= 64) attn_seq_kernel<2><<<(unsigned)grid, 256, 0, s>>>(a);
-    else if (a.Dh <= 96) attn_seq_kernel<3><<<(unsigned)grid, 256, 0, s>>>(a);
-    else attn_seq_kernel<4><<<(unsigned)grid, 256, 0, s>>>(a);
+    const int rc = paged ? launch<true>(a, (unsigned)grid, s) : launch<false>(a, (unsigned)grid, s);
+    if (rc) return rc;
   }
   if (a.ct) attn_seq_join_kernel<<<(unsigned)(((int64_t)a.T * a.H + 3) / 4), 256, 0, s>>>(a);
   return qie_last_error();

@@ -57,15 +57,6 @@ __global__ void __launch_bounds__(512) attn_seq_pp_kernel(SeqArgs a) {
   if (t0 > 0 && t0 >= ntot) return;  // a causal block that ends before this chunk
 
   bf16x8_t qf[KS];
-  {
-    const bf16_t* qr = a.q + (int64_t)(it.start + tok) * a.ldq + (int64_t)head * a.hsq + 8 * hf;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      qf[ks] = bf16x8_t{};
-      if (16 * ks + 8 * hf < a.Dh) qf[ks] = *(const bf16x8_t*)(qr + 16 * ks);
-    }
-  }
-
   f32x16_t s[2], o[ND];
   bf16x8_t pf[4];
   float m_run = kLow, l_run = 0.f;
@@ -270,14 +261,25 @@ __global__ void __launch_bounds__(512) attn_seq_pp_kernel(SeqArgs a) {
   using IA = std::integral_constant<int, NQ + NP>;
 
   if (t0 < ntiles) {
-    if constexpr (PAGED) pages(t0);
-    __builtin_amdgcn_s_waitcnt(0);  // q and the page ids: from here on the counter is the tiles'
+    if constexpr (PAGED) {
+      pages(t0);
+      __builtin_amdgcn_s_waitcnt(0);
+    }
     // K(t0 .. t0 + 2), V(t0), V(t0 + 1) resident; group 1 waits one phase
     dmaK(t0);
     if (t0 + 1 < ntiles) dmaK(t0 + 1);
     dmaV(t0);
     if (t0 + 2 < ntiles) dmaK(t0 + 2);
     if (t0 + 1 < ntiles) dmaV(t0 + 1);
+    {
+      const bf16_t* qr = a.q + (int64_t)(it.start + tok) * a.ldq + (int64_t)head * a.hsq + 8 * hf;
+  #pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        qf[ks] = bf16x8_t{};
+        if (16 * ks + 8 * hf < a.Dh) qf[ks] = *(const bf16x8_t*)(qr + 16 * ks);
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0);  // q as well: from here on the counter is the tiles'
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     if (grp == 1) asm volatile("s_barrier" ::: "memory");
     auto mend = [&]() { asm volatile("s_barrier" ::: "memory"); };

@@ -694,33 +694,43 @@ def silu_mul(gu: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tens
 
 
 # ---------------------------------------------------------------------------- sequences and their cache
-def _call_on(name: str, ref: torch.Tensor, *args) -> None:
-    """Launch on the current stream of the operands' device, which need not be the current one."""
-    if ref.device.index == torch.cuda.current_device():
-        _lib.call(name, *args, _stream())
+# Small calls are bound by the host: strides come from one stride() each, the stream from the raw getter.
+def _call_on(name: str, dev: int, *args) -> None:
+    """Launch on the current stream of device ``dev``, the operands', which need not be the current one."""
+    if dev == torch._C._cuda_getDevice():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with torch.cuda.device(ref.device):
-            _lib.call(name, *args, _stream())
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
-def _same_dev(ref: torch.Tensor, *ts):
-    for t in (ref, *ts):
-        _chk(t is None or (t.is_cuda and t.device == ref.device), "libqie ops need tensors of one device")
+def _same_dev(*ts) -> int:
+    """The one device of the tensors."""
+    dev = ts[0].get_device()
+    for t in ts:
+        if dev < 0 or (t is not None and t.get_device() != dev):
+            raise ValueError("libqie ops need tensors of one device")
+    return dev
 
 
-def _ld(t: torch.Tensor, width: int) -> int:
-    """Row stride of a row-major view; of a single row, whose stride says nothing, its width."""
-    return t.stride(0) if t.shape[0] > 1 else -(-width // 8) * 8
+def _rows2(t: torch.Tensor, width: int, align: int, name: str) -> int:
+    """Row stride of a bf16 row-major view [T, >= width]; of a single row, whose stride says nothing, its width."""
+    st = t.stride()
+    ld = st[0] if t.shape[0] > 1 else -(-width // 8) * 8
+    if t.dtype != BF16 or len(st) != 2 or st[1] != 1 or t.shape[1] < width or ld % align or t.data_ptr() % (2 * align):
+        raise ValueError(f"{name}: bf16 row-major [rows, >= {width}], rows aligned to {2 * align} bytes")
+    return ld
 
 
 def _rope_args(T: int, head_dim: int, positions, turns, axis):
     pairs = turns.numel()
-    _chk(positions.dtype == torch.int32 and positions.dim() == 2 and positions.shape[1] == T and
-         (T <= 1 or positions.stride(1) == 1), "positions int32 [axes, rows]")
+    st = positions.stride()
+    _chk(positions.dtype == torch.int32 and len(st) == 2 and positions.shape[1] == T and (T <= 1 or st[1] == 1),
+         "positions int32 [axes, rows]")
     _chk(turns.dtype == torch.float64 and turns.is_contiguous() and axis.dtype == torch.int32 and
          axis.is_contiguous() and axis.numel() == pairs, "turns float64 [pairs], axis int32 [pairs]")
     _chk(0 < 2 * pairs <= head_dim and pairs <= 128, "0 < 2 * pairs <= head_dim, pairs <= 128")
-    return (_p(positions), max(positions.stride(0), T), positions.shape[0], _p(turns), _p(axis), pairs)
+    return (positions.data_ptr(), max(st[0], T), positions.shape[0], turns.data_ptr(), axis.data_ptr(), pairs)
 
 
 def rope_axes(x: torch.Tensor, h0: int, nh: int, head_dim: int, positions: torch.Tensor, turns: torch.Tensor,
@@ -730,39 +740,37 @@ def rope_axes(x: torch.Tensor, h0: int, nh: int, head_dim: int, positions: torch
     pair i of a head turns by positions[axis[i]] * turns[i] full turns, positions int32 [axes, T]
     (``rope.section_turns`` / ``rope.axes_turns`` make turns and axis). Pairs are half a rotary width
     apart, or neighbours if ``interleaved``. In place, or into ``out`` [T, >= nh heads], whose first
-    head is head h0; one rounding, angles in 64 bits."""
-    _same_dev(x, positions, turns, axis, out)
+    head is head h0 and which does not overlap x; one rounding, angles in 64 bits."""
+    dev = _same_dev(x, positions, turns, axis, out)
     hs = head_dim if head_stride is None else head_stride
-    _chk(x.dtype == BF16 and _is2d_rowmajor(x), "bf16 row-major")
-    T = x.shape[0]
+    _chk(h0 >= 0 and nh >= 1 and hs >= head_dim and hs % 2 == 0, "heads, an even stride apart")
     width = (nh - 1) * hs + head_dim
-    _chk(h0 >= 0 and nh >= 1 and hs >= head_dim and h0 * hs + width <= x.shape[1], "heads exceed the row")
-    _chk(hs % 2 == 0 and (T <= 1 or x.stride(0) % 2 == 0), "even strides")
+    ldx = _rows2(x, h0 * hs + width, 2, "x")
+    T = x.shape[0]
     rope = _rope_args(T, head_dim, positions, turns, axis)
     xp = x.data_ptr() + 2 * h0 * hs
     if out is None:
-        op, ldo = xp, _ld(x, width)
+        op, ldo = xp, ldx
     else:
-        _chk(out.dtype == BF16 and _is2d_rowmajor(out) and out.shape[0] == T and out.shape[1] >= width and
-             (T <= 1 or out.stride(0) % 2 == 0), "out [T, heads]")
-        op, ldo = out.data_ptr(), _ld(out, width)
-    _chk(xp % 4 == 0 and op % 4 == 0, "4-byte aligned heads")
-    if T == 0:
-        return x if out is None else out
-    _call_on("qie_rope_axes_bf16", x, xp, _ld(x, width), op, ldo, T, nh, head_dim, hs, *rope, int(interleaved))
+        ldo = _rows2(out, width, 2, "out")
+        _chk(out.shape[0] == T, "out [T, heads]")
+        op = out.data_ptr()
+    if T:
+        _call_on("qie_rope_axes_bf16", dev, xp, ldx, op, ldo, T, nh, head_dim, hs, *rope, int(interleaved))
     return x if out is None else out
 
 
 def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, head_dim: int):
     """Checks of a cache's pages [pages, kv_heads, page_size, head_dim] -> their strides."""
-    _chk(k_pages.dtype == BF16 and v_pages.dtype == BF16 and k_pages.dim() == 4 and k_pages.shape == v_pages.shape and
-         k_pages.stride() == v_pages.stride(), "k_pages / v_pages: bf16 [pages, kv_heads, page_size, head_dim], same strides")
+    st = k_pages.stride()
+    _chk(k_pages.dtype == BF16 and v_pages.dtype == BF16 and len(st) == 4 and k_pages.shape == v_pages.shape and
+         st == v_pages.stride(), "k_pages / v_pages: bf16 [pages, kv_heads, page_size, head_dim], same strides")
     N, Hk, P, Dh = k_pages.shape
-    _chk(N > 0 and Hk > 0 and Dh == head_dim and Dh % 8 == 0 and k_pages.stride(3) == 1, "pages: rows of head_dim, a multiple of 8")
+    ps, hs, ss, one = st
+    _chk(N > 0 and Hk > 0 and Dh == head_dim and Dh % 8 == 0 and one == 1, "pages: rows of head_dim, a multiple of 8")
     _chk(16 <= P <= 1024 and P & (P - 1) == 0, "page_size: a power of two in [16, 1024]")
-    ps, hs, ss = k_pages.stride(0), k_pages.stride(1), k_pages.stride(2)
-    _chk(ps % 8 == 0 and hs % 8 == 0 and ss % 8 == 0 and ss >= Dh and (N == 1 or ps >= Dh) and (Hk == 1 or hs >= Dh) and
-         k_pages.data_ptr() % 16 == 0 and v_pages.data_ptr() % 16 == 0, "pages: 16-byte aligned rows that do not overlap")
+    _chk((ps | hs | ss) % 8 == 0 and ss >= Dh and (N == 1 or ps >= Dh) and (Hk == 1 or hs >= Dh) and
+         (k_pages.data_ptr() | v_pages.data_ptr()) % 16 == 0, "pages: 16-byte aligned rows that do not overlap")
     return N, Hk, P, ps, hs, ss
 
 
@@ -773,48 +781,52 @@ def rope_append(qkv: torch.Tensor, heads: int, kv_heads: int, head_dim: int, pos
     cache: the rotated q goes to ``out`` [T, heads * head_dim] (default: in place), the rotated k and
     v of row t to slot ``slots[t] % page_size`` of page ``slots[t] // page_size`` (int64; < 0 or past
     the pool: not stored; the slots of one call must be distinct). Returns the q rows."""
-    _same_dev(qkv, positions, turns, axis, k_pages, v_pages, slots, out)
-    _chk(qkv.dtype == BF16 and _is2d_rowmajor(qkv) and heads > 0 and kv_heads > 0, "bf16 row-major")
+    dev = _same_dev(qkv, positions, turns, axis, k_pages, v_pages, slots, out)
+    _chk(heads > 0 and kv_heads > 0, "heads")
+    ldx = _rows2(qkv, (heads + 2 * kv_heads) * head_dim, 8, "qkv")
     T = qkv.shape[0]
-    width = (heads + 2 * kv_heads) * head_dim
-    _chk(qkv.shape[1] >= width and qkv.data_ptr() % 16 == 0 and (T <= 1 or qkv.stride(0) % 8 == 0),
-         "qkv [T, (heads + 2 kv_heads) * head_dim], 16-byte aligned rows")
     N, Hk, P, ps, hs, ss = _pages(k_pages, v_pages, head_dim)
     _chk(Hk == kv_heads, "pages of another number of kv heads")
     _chk(slots.dtype == torch.int64 and slots.dim() == 1 and slots.numel() == T and slots.is_contiguous(), "slots int64 [T]")
     rope = _rope_args(T, head_dim, positions, turns, axis)
     if out is None:
         out = qkv[:, :heads * head_dim]
-    _chk(out.dtype == BF16 and _is2d_rowmajor(out) and tuple(out.shape) == (T, heads * head_dim) and
-         out.data_ptr() % 16 == 0 and (T <= 1 or out.stride(0) % 8 == 0), "out [T, heads * head_dim], 16-byte aligned rows")
-    if T == 0:
-        return out
-    _call_on("qie_rope_append_bf16", qkv, _p(qkv), _ld(qkv, width), _p(out), _ld(out, heads * head_dim), T, heads,
-             kv_heads, head_dim, *rope, int(interleaved), _p(k_pages), _p(v_pages), N, P, ps, hs, ss, _p(slots))
+        ldo = ldx
+    else:
+        ldo = _rows2(out, heads * head_dim, 8, "out")
+        _chk(tuple(out.shape) == (T, heads * head_dim), "out [T, heads * head_dim]")
+    if T:
+        _call_on("qie_rope_append_bf16", dev, qkv.data_ptr(), ldx, out.data_ptr(), ldo, T, heads, kv_heads, head_dim,
+                 *rope, int(interleaved), k_pages.data_ptr(), v_pages.data_ptr(), N, P, ps, hs, ss, slots.data_ptr())
     return out
 
 
 def _heads3(t: torch.Tensor, name: str):
     """(row stride, head stride) of a [T, heads, head_dim] view with 16-byte aligned heads."""
+    st = t.stride()
+    if len(st) != 3:
+        raise ValueError(name + ": [T, heads, head_dim]")
     T, H, Dh = t.shape
-    ld, hs = t.stride(0) if T > 1 else H * Dh, t.stride(1) if H > 1 else Dh
-    _chk(t.dtype == BF16 and t.stride(2) == 1 and ld % 8 == 0 and hs % 8 == 0 and t.data_ptr() % 16 == 0,
-         name + ": bf16 [T, heads, head_dim], 16-byte aligned heads")
+    ld, hs = st[0] if T > 1 else H * Dh, st[1] if H > 1 else Dh
+    if t.dtype != BF16 or st[2] != 1 or (ld | hs) % 8 or t.data_ptr() % 16:
+        raise ValueError(name + ": bf16 [T, heads, head_dim], 16-byte aligned heads")
     return ld, hs
 
 
-def _seq_args(q, out, head_dim_ok, scale):
-    _chk(q.dim() == 3 and q.shape[1] > 0, "q [T, heads, head_dim]")
-    T, H, Dh = q.shape
-    _chk(head_dim_ok and 0 < Dh <= 128 and Dh % 8 == 0, "head_dim: a multiple of 8, <= 128, the same everywhere")
+def _seq_args(q: torch.Tensor, out, scale):
+    """Strides of q and of out (made here if not given), the scale."""
+    ldq, hsq = _heads3(q, "q")
+    H, Dh = q.shape[1:]
+    _chk(H > 0 and 0 < Dh <= 128 and Dh % 8 == 0, "head_dim: a multiple of 8, <= 128")
     sc = 1.0 / math.sqrt(Dh) if scale is None else float(scale)
     _chk(0.0 < sc < math.inf, "scale must be positive and finite")
     if out is None:
-        out = torch.empty(T, H, Dh, dtype=BF16, device=q.device)
+        out = torch.empty(q.shape, dtype=BF16, device=q.device)
+        return out, sc, ldq, hsq, H * Dh, Dh
     _chk(out.shape == q.shape, "out [T, heads, head_dim]")
     ldo, hso = _heads3(out, "out")
     _chk(ldo >= Dh and hso >= Dh, "out: rows that do not overlap")
-    return out, sc, ldo, hso
+    return out, sc, ldq, hsq, ldo, hso
 
 
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -825,26 +837,26 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     ``causal``: key j <= query i. Views of one projection's columns are fine. A query's result holds
     nothing of the keys it does not see. Rows outside every sequence are left as they were (``out``
     given) or undefined."""
-    _same_dev(q, k, v, cu_seqlens, out)
-    _chk(k.dim() == 3 and k.shape == v.shape and k.shape[0] == q.shape[0], "k, v [T, kv_heads, head_dim]")
-    out, sc, ldo, hso = _seq_args(q, out, k.shape[2] == q.shape[-1], scale)
+    dev = _same_dev(q, k, v, cu_seqlens, out)
+    out, sc, ldq, hsq, ldo, hso = _seq_args(q, out, scale)
     T, H, Dh = q.shape
+    kst = _heads3(k, "k")
     Hk = k.shape[1]
-    _chk(Hk > 0 and H % Hk == 0, "heads must be a multiple of kv_heads")
-    _chk(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 2 and
-         cu_seqlens.is_contiguous(), "cu_seqlens int32 [seqs + 1]")
-    (ldq, hsq), kst, vst = _heads3(q, "q"), _heads3(k, "k"), _heads3(v, "v")
-    _chk(kst == vst and kst[0] >= Dh, "k and v: the same strides, rows that do not overlap")
-    if T == 0:
-        return out
-    _call_on("qie_attention_packed_bf16", q, _p(q), ldq, hsq, _p(k), _p(v), kst[0], kst[1], _p(cu_seqlens),
-             cu_seqlens.numel() - 1, T, H, Hk, Dh, int(causal), sc, _p(out), ldo, hso)
+    _chk(k.shape == v.shape and k.shape[0] == T and k.shape[2] == Dh and Hk > 0 and H % Hk == 0,
+         "k, v [T, kv_heads, head_dim], heads a multiple of kv_heads")
+    _chk(kst == _heads3(v, "v") and kst[0] >= Dh, "k and v: the same strides, rows that do not overlap")
+    B = cu_seqlens.numel() - 1
+    _chk(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and B >= 1 and cu_seqlens.is_contiguous(),
+         "cu_seqlens int32 [seqs + 1]")
+    if T:
+        _call_on("qie_attention_packed_bf16", dev, q.data_ptr(), ldq, hsq, k.data_ptr(), v.data_ptr(), kst[0], kst[1],
+                 cu_seqlens.data_ptr(), B, T, H, Hk, Dh, int(causal), sc, out.data_ptr(), ldo, hso)
     return out
 
 
 def attention_paged_workspace_bytes(tokens: int, seqs: int, heads: int, kv_heads: int, head_dim: int,
                                     table_width: int, page_size: int) -> int:
-    """Bytes that ``attention_paged(..., workspace=)`` needs (0: none)."""
+    """Bytes that ``attention_paged(..., workspace=)`` needs (0: none, as for tables of up to 1024 tokens)."""
     n = ctypes.c_int64(0)
     _lib.call("qie_attention_paged_workspace", tokens, seqs, heads, kv_heads, head_dim, table_width, page_size, ctypes.byref(n))
     return n.value
@@ -860,13 +872,14 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     page_table[b, j // page_size] (device int32 [seqs, width]; a page outside the pool reads as zeros)
     of k_pages, v_pages [pages, Hk, page_size, Dh]. ``workspace`` (>= attention_paged_workspace_bytes,
     not shared with a call that may run at the same time) is taken from torch's allocator if not given."""
-    _same_dev(q, k_pages, v_pages, page_table, kv_lens, cu_seqlens, out, workspace)
-    out, sc, ldo, hso = _seq_args(q, out, True, scale)
+    dev = _same_dev(q, k_pages, v_pages, page_table, kv_lens, cu_seqlens, out, workspace)
+    out, sc, ldq, hsq, ldo, hso = _seq_args(q, out, scale)
     T, H, Dh = q.shape
     N, Hk, P, ps, hs, ss = _pages(k_pages, v_pages, Dh)
     _chk(H % Hk == 0, "heads must be a multiple of kv_heads")
-    _chk(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.shape[0] > 0 and
-         page_table.shape[1] > 0 and page_table.stride(1) == 1, "page_table int32 [seqs, width]")
+    tst = page_table.stride()
+    _chk(page_table.dtype == torch.int32 and len(tst) == 2 and page_table.numel() > 0 and tst[1] == 1,
+         "page_table int32 [seqs, width]")
     B, W = page_table.shape
     _chk(kv_lens.dtype == torch.int32 and kv_lens.dim() == 1 and kv_lens.numel() == B and kv_lens.is_contiguous(),
          "kv_lens int32 [seqs]")
@@ -875,15 +888,17 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     else:
         _chk(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.numel() == B + 1 and
              cu_seqlens.is_contiguous(), "cu_seqlens int32 [seqs + 1]")
-    ldq, hsq = _heads3(q, "q")
     if T == 0:
         return out
-    need = attention_paged_workspace_bytes(T, B, H, Hk, Dh, W, P)
-    if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    have = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    _chk(have >= need and (workspace is None or workspace.is_contiguous()), "workspace too small")
-    _call_on("qie_attention_paged_bf16", q, _p(q), ldq, hsq, _p(k_pages), _p(v_pages), N, P, ps, hs, ss,
-             _p(page_table), max(page_table.stride(0), W), W, _p(kv_lens), _p(cu_seqlens), B, T, H, Hk, Dh, sc, _p(out),
-             ldo, hso, _p(workspace), have)
+    have = wp = 0
+    if W * P > 1024:
+        need = attention_paged_workspace_bytes(T, B, H, Hk, Dh, W, P)
+        if need and workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        if workspace is not None:
+            have, wp = workspace.numel() * workspace.element_size(), workspace.data_ptr()
+            _chk(have >= need and workspace.is_contiguous() and wp % 16 == 0, "workspace: contiguous, 16-byte aligned, large enough")
+    _call_on("qie_attention_paged_bf16", dev, q.data_ptr(), ldq, hsq, k_pages.data_ptr(), v_pages.data_ptr(), N, P, ps,
+             hs, ss, page_table.data_ptr(), max(tst[0], W), W, kv_lens.data_ptr(),
+             None if cu_seqlens is None else cu_seqlens.data_ptr(), B, T, H, Hk, Dh, sc, out.data_ptr(), ldo, hso, wp, have)
     return out
