@@ -134,14 +134,19 @@ __device__ __forceinline__ float quad_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// bf16 pairs with an infinity or NaN among them
-__device__ __forceinline__ bool nonfinite(const u32x4_t w) {
-  const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= (ww[i] & 0x7f80u) == 0x7f80u || (ww[i] & 0x7f800000u) == 0x7f800000u;
-  return bad;
-}
+// Infinities and NaN among bf16 values: the largest magnitude so far, as integers, one per half
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
+struct Magnitude {
+  u16x2_t m = {0, 0};
+  __device__ __forceinline__ void add(const bf16x8_t x) {
+    const u32x4_t w = __builtin_bit_cast(u32x4_t, x);
+    m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, w.x & 0x7fff7fffu));
+    m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, w.y & 0x7fff7fffu));
+    m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, w.z & 0x7fff7fffu));
+    m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, w.w & 0x7fff7fffu));
+  }
+  __device__ __forceinline__ bool nonfinite() const { return m.x >= 0x7f80 || m.y >= 0x7f80; }
+};
 // the finite values of a fragment, 0 for the others
 __device__ __forceinline__ bf16x8_t finite(bf16x8_t x) {
   const u32x4_t w = __builtin_bit_cast(u32x4_t, x);

@@ -175,13 +175,13 @@ __global__ void __launch_bounds__(256, NK == 4 ? 3 : 4) attn_seq_kernel(SeqArgs 
       return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
     };
     // 0 * inf and 0 * NaN: a masked key's V must not reach the rows that do not see it
-    bool bad = false;
+    Magnitude mag;
     if (masked) {
 #pragma unroll
-      for (int db = 0; db < ND; ++db) bad |= nonfinite(__builtin_bit_cast(u32x4_t, vfrag(db)));
+      for (int db = 0; db < ND; ++db) mag.add(vfrag(db));
       asm volatile("" ::: "memory");  // read again below: keeping all of them costs registers
     }
-    if (__builtin_expect(__any(bad), 0)) {
+    if (__builtin_expect(__any(mag.nonfinite()), 0)) {
       // the finite values as ever, then what a row sees of the others
 #pragma unroll
       for (int db = 0; db < ND; ++db) {

@@ -178,13 +178,13 @@ __global__ void __launch_bounds__(64 * NW) attn_seq_few_kernel(SeqArgs a) {
       const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t QIE_LDS*)(p0 + 16 * kRowB));
       return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
     };
-    bool bad = false;  // 0 * inf and 0 * NaN: a masked key's V must not reach the rows that do not see it
+    Magnitude mag;  // 0 * inf and 0 * NaN: a masked key's V must not reach the rows that do not see it
     if (masked) {
 #pragma unroll
-      for (int db = 0; db < ND; ++db) bad |= nonfinite(__builtin_bit_cast(u32x4_t, vfrag(db)));
+      for (int db = 0; db < ND; ++db) mag.add(vfrag(db));
       asm volatile("" ::: "memory");
     }
-    if (__builtin_expect(__any(bad), 0)) {
+    if (__builtin_expect(__any(mag.nonfinite()), 0)) {
 #pragma unroll
       for (int db = 0; db < ND; ++db) {
         const bf16x8_t A = finite(vfrag(db));

@@ -214,14 +214,14 @@ __global__ void __launch_bounds__(512) attn_seq_pp_kernel(SeqArgs a) {
     l_run += ps0 + ps1;
     done = false;
     if (masked) {  // V(t) landed a phase ago: are there infinities or NaN that a row must not see?
-      bool bad = false;
+      Magnitude mag;
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
 #pragma unroll
-        for (int db = 0; db < ND; ++db) bad |= nonfinite(__builtin_bit_cast(u32x4_t, vfrag(ks, db, t)));
+        for (int db = 0; db < ND; ++db) mag.add(vfrag(ks, db, t));
         asm volatile("" ::: "memory");  // few fragments in registers at a time
       }
-      if (__builtin_expect(__any(bad), 0)) {
+      if (__builtin_expect(__any(mag.nonfinite()), 0)) {
         done = true;  // O += V P here: the finite values, then what a row sees of the others
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
