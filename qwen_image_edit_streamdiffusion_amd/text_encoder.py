@@ -15,6 +15,11 @@ carry the residual add in their epilogue), RMSNorm / RoPE / SwiGLU / embedding a
 attention runs all heads per launch: head-batched fp32 score GEMM (GQA: the kv operand advances once
 per group), one causal softmax over every head's rows, head-batched P.V against V^T (prompt
 lengths are a few hundred tokens, so the full score blocks stay small).
+
+``forward_packed`` takes several prompts in one pass without padding (ops.rope_axes,
+ops.attention_packed: no scores in memory), ``extend`` new tokens after what a PagedKVCache holds of
+their sequences (ops.rope_append, ops.attention_paged). Their rotation has one rounding, fp32 angles
+and tables none; ``packed_attention`` makes ``forward`` go the same way.
 """
 from __future__ import annotations
 
@@ -22,11 +27,13 @@ import hashlib
 import math
 from collections import OrderedDict
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
 from . import ops
+from .kv_cache import PagedKVCache
+from .rope import section_turns
 
 BF16 = torch.bfloat16
 
@@ -149,9 +156,10 @@ class EncoderLinears:
 class QwenVLTextModel:
     """``Qwen2_5_VLTextModel`` forward on the HIP path (one prompt at a time: no padding mask)."""
 
-    def __init__(self, config: Optional[TextEncoderConfig] = None, device="cuda"):
+    def __init__(self, config: Optional[TextEncoderConfig] = None, device="cuda", packed_attention: bool = False):
         self.config = config or TextEncoderConfig()
         self.device = torch.device(device)
+        self.packed_attention = packed_attention
         c = self.config
         if c.head_dim % 64 or c.hidden_size % 64 or c.intermediate_size % 64:
             raise NotImplementedError("head_dim, hidden_size and intermediate_size must be multiples of 64")
@@ -160,6 +168,7 @@ class QwenVLTextModel:
         self.layers: List[Dict[str, torch.Tensor]] = []
         self.w: Dict[str, torch.Tensor] = {}
         self.lin = EncoderLinears(self.device)
+        self.turns, self.axis = section_turns(c.mrope_section, c.rope_theta, self.device)
 
     # ------------------------------------------------------------------ weights
     @staticmethod
@@ -204,6 +213,9 @@ class QwenVLTextModel:
         c, w, dev = self.config, self.w, self.device
         if not self.layers:
             raise RuntimeError("text encoder weights not loaded")
+        if self.packed_attention:
+            return self.forward_packed([input_ids if inputs_embeds is None else inputs_embeds],
+                                       None if position_ids is None else [position_ids])[0]
         D, H, Hk, Dh, F = c.hidden_size, c.num_attention_heads, c.num_key_value_heads, c.head_dim, c.intermediate_size
         S = int(input_ids.numel()) if inputs_embeds is None else int(inputs_embeds.shape[0])
         Sp = -(-S // 64) * 64  # padded rows: GEMM N / K alignment; causal masking keeps rows < S exact
@@ -250,6 +262,89 @@ class QwenVLTextModel:
 
     __call__ = forward
 
+    # ------------------------------------------------------------------ several prompts, new tokens
+    def new_cache(self, pages: int, page_size: int = 64) -> PagedKVCache:
+        """An empty cache of this model's layers (``extend``)."""
+        c = self.config
+        return PagedKVCache(c.num_hidden_layers, c.num_key_value_heads, c.head_dim, pages, page_size, self.device)
+
+    def forward_packed(self, prompts: Sequence[torch.Tensor],
+                       position_ids: Optional[Sequence[torch.Tensor]] = None) -> List[torch.Tensor]:
+        """Several prompts in one pass: token ids [S_i] or embeddings [S_i, D] each, positions [3, S_i]
+        (default: 0..S_i-1 on all three axes) -> their last hidden states [S_i, D], as ``forward`` of each."""
+        lens = [int(p.shape[0]) if p.is_floating_point() else int(p.numel()) for p in prompts]
+        if position_ids is None:
+            position_ids = [torch.arange(n).view(1, n).expand(3, n) for n in lens]
+        cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32).to(self.device)
+        H, Hk, Dh = self.config.num_attention_heads, self.config.num_key_value_heads, self.config.head_dim
+
+        def attend(layer, qkv, q3, pos, out):
+            ops.rope_axes(qkv, 0, H + Hk, Dh, pos, self.turns, self.axis)
+            kv = qkv[:, H * Dh:].unflatten(1, (2, Hk, Dh))
+            ops.attention_packed(q3, kv[:, 0], kv[:, 1], cu, out=out)
+
+        return list(self._rows(prompts, position_ids, lens, attend).split(lens))
+
+    def extend(self, cache: PagedKVCache, seqs: Sequence[int], tokens: Sequence[torch.Tensor],
+               position_ids: Optional[Sequence[torch.Tensor]] = None) -> List[torch.Tensor]:
+        """New tokens (ids [n_i] or embeddings [n_i, D]) of sequences of ``cache``, behind what it holds of
+        them: their last hidden states [n_i, D], as the rows that ``forward`` of the whole sequences gives.
+        positions [3, n_i] (default: counted on from the sequence's length)."""
+        lens = [int(p.shape[0]) if p.is_floating_point() else int(p.numel()) for p in tokens]
+        if position_ids is None:
+            position_ids = [torch.arange(cache.length(s), cache.length(s) + n).view(1, n).expand(3, n)
+                            for s, n in zip(seqs, lens)]
+        st = cache.step(seqs, lens)
+        c = self.config
+        H, Hk, Dh = c.num_attention_heads, c.num_key_value_heads, c.head_dim
+        nb = ops.attention_paged_workspace_bytes(sum(lens), len(lens), H, Hk, Dh, st.page_table.shape[1], cache.page_size)
+        ws = torch.empty(nb, dtype=torch.uint8, device=self.device) if nb else None
+
+        def attend(layer, qkv, q3, pos, out):
+            k, v = cache.k[layer], cache.v[layer]
+            ops.rope_append(qkv, H, Hk, Dh, pos, self.turns, self.axis, k, v, st.slots)
+            ops.attention_paged(q3, k, v, st.page_table, st.kv_lens, cu_seqlens=st.cu_seqlens, out=out, workspace=ws)
+
+        return list(self._rows(tokens, position_ids, lens, attend).split(lens))
+
+    def _rows(self, prompts, position_ids, lens, attend) -> torch.Tensor:
+        """The layers over the rows of all sequences, one behind the other; ``attend(layer, qkv, q, positions, out)``
+        rotates the rows' heads and fills out [T, H, Dh]."""
+        c, w, dev = self.config, self.w, self.device
+        if not self.layers:
+            raise RuntimeError("text encoder weights not loaded")
+        D, H, Hk, Dh, F = c.hidden_size, c.num_attention_heads, c.num_key_value_heads, c.head_dim, c.intermediate_size
+        T = sum(lens)
+        if len(position_ids) != len(lens) or any(tuple(p.shape) != (3, n) for p, n in zip(position_ids, lens)):
+            raise ValueError("positions [3, tokens] for each sequence")
+        h = torch.empty(T, D, dtype=BF16, device=dev)
+        if T == 0:
+            return h
+        pos = torch.cat([p.cpu() for p in position_ids], 1).to(torch.int32).to(dev)
+        x = torch.empty(T, D, dtype=BF16, device=dev)
+        at = 0
+        for p, n in zip(prompts, lens):
+            if p.is_floating_point():
+                x[at:at + n] = p.to(dev).to(BF16)
+            elif n:
+                ops.embed_rows(w["embed"], p.reshape(-1).to(dev).to(torch.int32), out=x[at:at + n])
+            at += n
+        qkv = torch.empty(T, (H + 2 * Hk) * Dh, dtype=BF16, device=dev)
+        att = torch.empty(T, H * Dh, dtype=BF16, device=dev)
+        q3, out = qkv[:, :H * Dh].unflatten(1, (H, Dh)), att.view(T, H, Dh)
+        gu = torch.empty(T, 2 * F, dtype=BF16, device=dev)
+        a = torch.empty(T, F, dtype=BF16, device=dev)
+        for i, L in enumerate(self.layers):
+            ops.rmsnorm(x, L["ln1"], out=h, eps=c.rms_norm_eps)
+            self.lin.linear(h, L["w_qkv"], L["b_qkv"], qkv)
+            attend(i, qkv, q3, pos, out)
+            self.lin.residual(att, L["w_o"], w["zero_d"], w["ones"], x)
+            ops.rmsnorm(x, L["ln2"], out=h, eps=c.rms_norm_eps)
+            self.lin.linear(h, L["w_gu"], w["zero_2f"], gu)
+            ops.silu_mul(gu, out=a)
+            self.lin.residual(a, L["w_down"], w["zero_d"], w["ones"], x)
+        return ops.rmsnorm(x, w["norm"], out=h, eps=c.rms_norm_eps)
+
 
 # ---------------------------------------------------------------------------- text + vision
 def rope_index(input_ids: torch.Tensor, image_token_id: int, image_grid_thw=None, spatial_merge_size: int = 2
@@ -290,6 +385,15 @@ def rope_index(input_ids: torch.Tensor, image_token_id: int, image_grid_thw=None
     return pos
 
 
+@dataclass
+class _Prefix:
+    """A prompt whose k / v the cache holds: its tokens, its pictures' key, its last hidden states."""
+
+    ids: torch.Tensor
+    key: Optional[tuple]
+    hidden: torch.Tensor
+
+
 class QwenVLEncoder:
     """``Qwen2_5_VLModel`` (vision tower + language model) as the reference's pipeline calls it
     for prompt embeddings: image embeddings scattered over the ``<|image_pad|>`` tokens, 3-D
@@ -298,10 +402,20 @@ class QwenVLEncoder:
     IMAGE_TOKEN_ID = 151655  # <|image_pad|> in the Qwen2.5-VL vocabulary
 
     def __init__(self, text_config: Optional[TextEncoderConfig] = None, vision_config=None, device="cuda",
-                 image_token_id: int = IMAGE_TOKEN_ID, vision_cache_size: int = 8):
+                 image_token_id: int = IMAGE_TOKEN_ID, vision_cache_size: int = 8, packed_attention: bool = False,
+                 prefix_cache_size: int = 0, prefix_cache_pages: Optional[int] = None):
+        """``packed_attention``: both models attend without a score matrix in memory, and several prompts
+        share a pass (``forward_batch``). ``prefix_cache_size`` > 0: the k / v of the last prompts are kept
+        (``prefix_cache_pages`` pages of 64 tokens, default 16 for each and one more), and a prompt that begins like one
+        of them -- the template and the same picture -- runs only the tokens behind what they share."""
         from .vision import QwenVLVisionTower, VisionConfig
-        self.text = QwenVLTextModel(text_config, device)
-        self.vision = QwenVLVisionTower(vision_config or VisionConfig(), device)
+        self.text = QwenVLTextModel(text_config, device, packed_attention)
+        self.vision = QwenVLVisionTower(vision_config or VisionConfig(), device, packed_attention)
+        self.packed_attention = packed_attention
+        self.prefix_cache_size = prefix_cache_size
+        self.prefix_pages = prefix_cache_pages or 16 * (prefix_cache_size + 1)
+        self.prefixes: "OrderedDict[int, _Prefix]" = OrderedDict()  # cache sequence -> what it holds
+        self.kv: Optional[PagedKVCache] = None
         if self.vision.config.out_hidden_size != self.text.config.hidden_size:
             raise ValueError("vision out_hidden_size must equal the text hidden_size")
         self.image_token_id = image_token_id
@@ -313,6 +427,7 @@ class QwenVLEncoder:
         self.vision_cache_size = vision_cache_size
 
     def load_state_dict(self, sd: Dict[str, torch.Tensor]) -> "QwenVLEncoder":
+        self.clear_prefixes()
         self.text.load_state_dict({k: v for k, v in sd.items() if "visual." not in k})
         self.vision.load_state_dict({k: v for k, v in sd.items() if "visual." in k})
         return self
@@ -320,7 +435,21 @@ class QwenVLEncoder:
     def forward(self, input_ids: torch.Tensor, pixel_values: Optional[torch.Tensor] = None,
                 image_grid_thw=None) -> torch.Tensor:
         """One prompt: input_ids [S] (or [1, S]) -> hidden states [S, D] bf16."""
-        ids = input_ids.reshape(-1)
+        if self.prefix_cache_size > 0:
+            return self._forward_prefix(input_ids.reshape(-1), pixel_values, image_grid_thw)
+        emb, pos = self._embeds(input_ids.reshape(-1), pixel_values, image_grid_thw)
+        return self.text(inputs_embeds=emb, position_ids=pos)
+
+    __call__ = forward
+
+    def forward_batch(self, prompts: Sequence[tuple]) -> List[torch.Tensor]:
+        """Several prompts, (input_ids, pixel_values or None, image_grid_thw or None) each, in one pass of the
+        language model -> their hidden states [S_i, D]."""
+        rows = [self._embeds(ids.reshape(-1), pv, grid) for ids, pv, grid in prompts]
+        return self.text.forward_packed([e for e, _ in rows], [p for _, p in rows])
+
+    def _embeds(self, ids: torch.Tensor, pixel_values, image_grid_thw):
+        """(embeddings [S, D] with the image rows spliced in, positions [3, S]) of one prompt."""
         dev = self.device
         S = ids.numel()
         Sp = -(-S // 64) * 64
@@ -334,19 +463,79 @@ class QwenVLEncoder:
             if where.numel() != img.shape[0]:
                 raise ValueError(f"{where.numel()} image tokens but {img.shape[0]} image embeddings")
             emb[where.to(dev)] = img  # masked_scatter of the image rows
-        pos = rope_index(ids, self.image_token_id, image_grid_thw if pixel_values is not None else None,
-                         self.vision.config.spatial_merge_size)
-        return self.text(inputs_embeds=emb[:S], position_ids=pos)
+        return emb[:S], self._positions(ids, pixel_values, image_grid_thw)
 
-    __call__ = forward
+    def _positions(self, ids, pixel_values, image_grid_thw) -> torch.Tensor:
+        return rope_index(ids, self.image_token_id, image_grid_thw if pixel_values is not None else None,
+                          self.vision.config.spatial_merge_size)
+
+    # ------------------------------------------------------------------ prompts that begin alike
+    def clear_prefixes(self) -> None:
+        """Forget the kept prompts (after a change of weights; load_state_dict does it)."""
+        for seq in self.prefixes:
+            self.kv.drop(seq)
+        self.prefixes.clear()
+
+    def _forward_prefix(self, ids: torch.Tensor, pixel_values, image_grid_thw) -> torch.Tensor:
+        ids = ids.cpu()
+        S = ids.numel()
+        key = None if pixel_values is None else self._vision_key(pixel_values, image_grid_thw)[0]
+        image = (ids == self.image_token_id).nonzero().view(-1)
+        best, common = None, 0
+        for seq, p in reversed(self.prefixes.items()):  # of equals, the one used last
+            m = min(S, p.ids.numel())
+            ne = (ids[:m] != p.ids[:m]).nonzero()
+            n = int(ne[0]) if ne.numel() else m
+            if p.key != key and image.numel():  # other pictures: the text before the first one is shared
+                n = min(n, int(image[0]))
+            if n > common:
+                best, common = seq, n
+        if best is not None:
+            self.prefixes.move_to_end(best)
+            if common == S:
+                return self.prefixes[best].hidden[:S]
+        pos = self._positions(ids, pixel_values, image_grid_thw)
+        if image.numel() and int(image[-1]) >= common:
+            new = self._embeds(ids, pixel_values, image_grid_thw)[0][common:]
+        else:
+            new = ids[common:]  # every image row lies in what is shared
+        if self.kv is None:
+            self.kv = self.text.new_cache(self.prefix_pages)
+        # room: the new sequence's pages beside the shared ones, older prompts go first
+        need = -(-S // self.kv.page_size) - common // self.kv.page_size
+        while self.kv.free_pages < need and self.prefixes and next(iter(self.prefixes)) != best:
+            old, _ = self.prefixes.popitem(last=False)
+            self.kv.drop(old)
+        if self.kv.free_pages < need:
+            emb = self._embeds(ids, pixel_values, image_grid_thw)[0]
+            return self.text.forward_packed([emb], [pos])[0]  # longer than the cache: not kept
+        seq = self.kv.fork(best, common) if common else self.kv.add()
+        try:
+            hidden = self.text.extend(self.kv, [seq], [new], [pos[:, common:]])[0]
+        except Exception:
+            self.kv.drop(seq)
+            raise
+        if common:
+            hidden = torch.cat([self.prefixes[best].hidden[:common], hidden])
+        self.prefixes[seq] = _Prefix(ids, key, hidden)
+        while len(self.prefixes) > self.prefix_cache_size:
+            old, _ = self.prefixes.popitem(last=False)
+            self.kv.drop(old)
+        return hidden
+
+    def _vision_key(self, pixel_values: torch.Tensor, image_grid_thw):
+        """(grid and content digest, grid) of a prompt's pictures."""
+        grid = tuple(tuple(int(v) for v in g) for g in (image_grid_thw.tolist() if torch.is_tensor(image_grid_thw)
+                                                         else image_grid_thw))
+        pv = pixel_values.detach().to("cpu", torch.float32).contiguous()
+        return (grid, hashlib.blake2b(pv.numpy().tobytes(), digest_size=16).hexdigest()), grid
 
     def _vision(self, pixel_values: torch.Tensor, image_grid_thw) -> torch.Tensor:
         grid = tuple(tuple(int(v) for v in g) for g in (image_grid_thw.tolist() if torch.is_tensor(image_grid_thw)
                                                          else image_grid_thw))
         if self.vision_cache_size <= 0:
             return self.vision.forward(pixel_values, grid)
-        pv = pixel_values.detach().to("cpu", torch.float32).contiguous()
-        key = (grid, hashlib.blake2b(pv.numpy().tobytes(), digest_size=16).hexdigest())
+        key, _ = self._vision_key(pixel_values, grid)
         hit = self.vision_cache.get(key)
         if hit is not None:
             self.vision_cache.move_to_end(key)
@@ -435,15 +624,20 @@ class QwenImageEditPromptEncoder:
     def _encode(self, prompts, image):
         imgs = self._condition_images(image)
         prefix = "".join(IMAGE_PROMPT_TEMPLATE.format(i + 1) for i in range(len(imgs)))
-        rows = []
+        inputs = []
         for p in prompts:
             kw = {"images": imgs} if imgs else {}
             mi = self.processor(text=[PROMPT_TEMPLATE.format(prefix + p)], return_tensors="pt", **kw)
             ids = mi["input_ids"][0]
             if "attention_mask" in mi:
                 ids = ids[mi["attention_mask"][0].bool()]
-            h = self.encoder(ids, mi.get("pixel_values"), mi.get("image_grid_thw"))
-            rows.append(h[self.drop:])
+            inputs.append((ids, mi.get("pixel_values"), mi.get("image_grid_thw")))
+        enc = self.encoder
+        if len(inputs) > 1 and getattr(enc, "packed_attention", False) and not enc.prefix_cache_size:
+            rows = enc.forward_batch(inputs)  # one pass over all prompts
+        else:
+            rows = [enc(*i) for i in inputs]
+        rows = [h[self.drop:] for h in rows]
         L = max(r.shape[0] for r in rows)
         D = rows[0].shape[1]
         embeds = torch.zeros(len(rows), L, D, dtype=BF16, device=rows[0].device)

@@ -25,6 +25,7 @@ from typing import Dict, List, Sequence, Tuple
 import torch
 
 from . import ops
+from .rope import axes_turns
 
 BF16 = torch.bfloat16
 
@@ -155,9 +156,12 @@ class QwenVLVisionTower:
 
     SLOT = 128  # zero-padded head slot
 
-    def __init__(self, config: VisionConfig = None, device="cuda"):
+    def __init__(self, config: VisionConfig = None, device="cuda", packed_attention: bool = False):
+        """``packed_attention``: windows and images as packed sequences (ops.rope_axes, ops.attention_packed on
+        the heads' own width), no score matrix in memory."""
         self.config = config or VisionConfig()
         self.device = torch.device(device)
+        self.packed_attention = packed_attention
         c = self.config
         if c.hidden_size % 64 or c.out_hidden_size % 64 or c.head_dim > self.SLOT or c.head_dim % 2:
             raise NotImplementedError("hidden sizes must be multiples of 64 and head_dim <= 128")
@@ -235,9 +239,18 @@ class QwenVLVisionTower:
         rows = (perm[:, None] * unit + torch.arange(unit)).reshape(-1)
         rows_dev = rows.to(torch.int32).to(dev)
         inv_dev = torch.argsort(perm).to(torch.int32).to(dev)
-        cos, sin = (t.to(dev) for t in rotary_tables(c, grid, perm, Sp))
-        rng_win = _row_ranges(cu_win, S, Sp).to(dev)
-        rng_full = _row_ranges(frame_seqlens(grid), S, Sp).to(dev)
+        packed = self.packed_attention
+        if packed:
+            pos = torch.zeros(2, Sp, dtype=torch.int32)
+            pos[:, :S] = vision_position_ids(grid, m)[rows].T
+            pos = pos.to(dev)
+            turns, axis = axes_turns((Dh // 2, Dh // 2), 10000.0, dev)
+            cu_win_dev = torch.tensor(cu_win, dtype=torch.int32).to(dev)
+            cu_full_dev = torch.tensor(frame_seqlens(grid), dtype=torch.int32).to(dev)
+        else:
+            cos, sin = (t.to(dev) for t in rotary_tables(c, grid, perm, Sp))
+            rng_win = _row_ranges(cu_win, S, Sp).to(dev)
+            rng_full = _row_ranges(frame_seqlens(grid), S, Sp).to(dev)
 
         xin = torch.zeros(Sp, self.Kp, dtype=BF16, device=dev)
         xin[:S, :c.patch_dim] = pixel_values.to(dev).to(BF16)
@@ -246,22 +259,31 @@ class QwenVLVisionTower:
         ops.embed_rows(x0, rows_dev, out=x[:S])  # window order
         h = torch.empty(Sp, D, dtype=BF16, device=dev)
         qkv = torch.empty(Sp, 3 * H * SL, dtype=BF16, device=dev)
-        att = torch.empty(Sp, H * SL, dtype=BF16, device=dev)
-        s = torch.empty(H * Sp, Sp, dtype=torch.float32, device=dev)  # all heads' scores
-        p = torch.empty(H * Sp, Sp, dtype=BF16, device=dev)
-        vt = torch.empty(H * SL, Sp, dtype=BF16, device=dev)
+        if packed:  # the slots' padding and the padding rows stay zero
+            att = torch.zeros(Sp, H * SL, dtype=BF16, device=dev)
+            q3, k3, v3 = (qkv.view(Sp, 3, H, SL)[:S, j, :, :Dh] for j in range(3))
+            out3 = att.view(Sp, H, SL)[:S, :, :Dh]
+        else:
+            att = torch.empty(Sp, H * SL, dtype=BF16, device=dev)
+            s = torch.empty(H * Sp, Sp, dtype=torch.float32, device=dev)  # all heads' scores
+            p = torch.empty(H * Sp, Sp, dtype=BF16, device=dev)
+            vt = torch.empty(H * SL, Sp, dtype=BF16, device=dev)
         gu = torch.empty(Sp, 2 * self.Fp, dtype=BF16, device=dev)
         a = torch.empty(Sp, self.Fp, dtype=BF16, device=dev)
         scale = Dh ** -0.5
         for i, B in enumerate(self.blocks):
-            rng = rng_full if i in c.fullatt_block_indexes else rng_win
+            full = i in c.fullatt_block_indexes
             ops.rmsnorm(x, B["n1"], out=h, eps=c.rms_norm_eps)
             self.lin.linear(h, B["w_qkv"], B["b_qkv"], qkv)
-            ops.rope_half(qkv, 0, 2 * H, Dh, cos, sin, head_stride=SL)
-            ops.transpose(qkv[:, 2 * H * SL:], out=vt)
-            ops.matmul_heads(qkv[:, :SL], SL, qkv[:, H * SL:(H + 1) * SL], SL, s[:Sp], Sp * Sp, H)
-            ops.softmax_rows(s, scale, out=p, ranges=rng)
-            ops.matmul_heads(p[:Sp], Sp * Sp, vt[:SL], SL * Sp, att[:, :SL], SL, H, bias=w["zero_slot"])
+            if packed:
+                ops.rope_axes(qkv, 0, 2 * H, Dh, pos, turns, axis, head_stride=SL)
+                ops.attention_packed(q3, k3, v3, cu_full_dev if full else cu_win_dev, causal=False, out=out3)
+            else:
+                ops.rope_half(qkv, 0, 2 * H, Dh, cos, sin, head_stride=SL)
+                ops.transpose(qkv[:, 2 * H * SL:], out=vt)
+                ops.matmul_heads(qkv[:, :SL], SL, qkv[:, H * SL:(H + 1) * SL], SL, s[:Sp], Sp * Sp, H)
+                ops.softmax_rows(s, scale, out=p, ranges=rng_full if full else rng_win)
+                ops.matmul_heads(p[:Sp], Sp * Sp, vt[:SL], SL * Sp, att[:, :SL], SL, H, bias=w["zero_slot"])
             self.lin.residual(att, B["w_proj"], B["b_proj"], w["ones"], x)
             ops.rmsnorm(x, B["n2"], out=h, eps=c.rms_norm_eps)
             self.lin.linear(h, B["w_gu"], B["b_gu"], gu)

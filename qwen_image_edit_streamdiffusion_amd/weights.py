@@ -331,9 +331,10 @@ def _prompt_encoder_configs(path: str):
     return tc, vc, img
 
 
-def load_prompt_encoder(path: str, device="cuda"):
+def load_prompt_encoder(path: str, device="cuda", **kwargs):
     """QwenVLEncoder (Qwen2.5-VL vision tower + language model) from a diffusers snapshot's
-    ``text_encoder/`` (config.json + safetensors shards; ``lm_head`` is skipped unread)."""
+    ``text_encoder/`` (config.json + safetensors shards; ``lm_head`` is skipped unread). ``kwargs``:
+    the encoder's own (``packed_attention=``, ``prefix_cache_size=``, ...)."""
     from safetensors import safe_open
     from .text_encoder import QwenVLEncoder
     files = sorted(glob.glob(os.path.join(path, "text_encoder", "*.safetensors"))) if os.path.isdir(path) else []
@@ -346,4 +347,4 @@ def load_prompt_encoder(path: str, device="cuda"):
             for k in fh.keys():
                 if not k.startswith("lm_head"):
                     sd[k] = fh.get_tensor(k)
-    return QwenVLEncoder(tc, vc, device, image_token_id=img).load_state_dict(sd)
+    return QwenVLEncoder(tc, vc, device, image_token_id=img, **kwargs).load_state_dict(sd)

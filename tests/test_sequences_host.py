@@ -96,3 +96,50 @@ def test_entry_points_refuse_on_the_host(lib):
     assert lib.qie_attention_paged_workspace(4, 1, 4, 1, 128, 1, 16, ctypes.byref(n)) == 0 and n.value == 0
     assert lib.qie_attention_paged_workspace(4, 1, 4, 1, 128, 4096, 16, ctypes.byref(n)) == 0 and n.value > 0
     assert lib.qie_attention_paged_workspace(4, 1, 4, 1, 128, 4096, 16, None) == -1
+
+
+# ---------------------------------------------------------------------------- the cache's pages
+def _cache(pages=8):
+    from qwen_image_edit_streamdiffusion_amd.kv_cache import PagedKVCache
+    return PagedKVCache(2, 1, 64, pages, 16, "cpu")
+
+
+def test_paged_cache_steps_and_pages():
+    c = _cache()
+    a, b = c.add(), c.add()
+    st = c.step([a, b], [20, 1])
+    assert c.free_pages == 5 and c.length(a) == 20 and c.length(b) == 1
+    assert st.kv_lens.tolist() == [20, 1] and st.cu_seqlens.tolist() == [0, 20, 21] and st.page_table.shape == (2, 2)
+    t = st.page_table
+    want = [int(t[0, i // 16]) * 16 + i % 16 for i in range(20)] + [int(t[1, 0]) * 16]
+    assert st.slots.tolist() == want and len(set(want)) == 21
+    st2 = c.step([b, a], [0, 12])  # a's second page fills up to its end
+    assert c.free_pages == 5 and st2.kv_lens.tolist() == [1, 32] and st2.slots.numel() == 12
+    assert st2.slots.tolist() == [int(t[0, 1]) * 16 + i for i in range(4, 16)]
+    c.drop(a)
+    assert c.free_pages == 7
+    with pytest.raises(KeyError):
+        c.length(a)
+
+
+def test_paged_cache_shared_pages_and_refusals():
+    from qwen_image_edit_streamdiffusion_amd.kv_cache import CacheFull, PagedKVCache
+    c = _cache(4)
+    a = c.add()
+    c.step([a], [40])  # three pages
+    f = c.fork(a, 32)  # two of them shared
+    assert c.free_pages == 1 and c.length(f) == 32
+    with pytest.raises(CacheFull):
+        c.step([a, f], [16, 1])
+    assert c.length(a) == 40 and c.length(f) == 32 and c.free_pages == 1  # a refused step changes nothing
+    st = c.step([f, a], [3, 2])
+    assert st.page_table[0, :2].tolist() == st.page_table[1, :2].tolist()
+    assert int(st.page_table[0, 2]) != int(st.page_table[1, 2])
+    c.drop(a)
+    assert c.free_pages == 1  # the shared pages stay with the fork
+    c.drop(f)
+    assert c.free_pages == 4
+    for bad in (lambda: c.fork(c.add(), 1), lambda: c.step([], []), lambda: c.step([1, 1], [1, 1]),
+                lambda: PagedKVCache(1, 1, 64, 4, 24, "cpu"), lambda: PagedKVCache(1, 1, 60, 4, 16, "cpu")):
+        with pytest.raises((ValueError, KeyError)):
+            bad()

@@ -1,6 +1,7 @@
 """Time the prompt encoder at Qwen2.5-VL-7B size on random bf16 weights: the
 vision tower on one 392x392 condition image (28x28 patches -> 196 image tokens) and the language
-model on the Edit-Plus prompt around it (S tokens). Prints one JSON line."""
+model on the Edit-Plus prompt around it (S tokens); both again on packed attention, four prompts one by
+one and in one pass, and a new instruction behind the cached template and picture. Prints one JSON line."""
 import argparse
 import json
 import os
@@ -35,9 +36,7 @@ def main():
     grid = [(1, a.grid, a.grid)]
     pv = torch.randn(a.grid * a.grid, vc.patch_dim)
     res = {}
-    for name, fn in (("vision", lambda: enc.vision(pv, grid)),
-                     ("text", lambda: enc.text(ids)),
-                     ("encoder", lambda: enc(ids, pv, grid))):
+    def timed(name, fn):
         fn()
         torch.cuda.synchronize()
         t0 = time.perf_counter()
@@ -45,6 +44,26 @@ def main():
             fn()
         torch.cuda.synchronize()
         res[name + "_ms"] = round((time.perf_counter() - t0) / a.iters * 1e3, 2)
+
+    timed("vision", lambda: enc.vision(pv, grid))
+    timed("text", lambda: enc.text(ids))
+    timed("encoder", lambda: enc(ids, pv, grid))
+    four = [torch.randint(0, 150000, (n,)) for n in (S, S // 2, S, S // 3)]
+    timed("text_4_prompts", lambda: [enc.text(i) for i in four])
+    enc.vision.packed_attention = enc.text.packed_attention = True
+    timed("vision_packed", lambda: enc.vision(pv, grid))
+    timed("text_packed", lambda: enc.text(ids))
+    timed("text_4_prompts_packed", lambda: enc.text.forward_packed(four))
+    cache = enc.text.new_cache(2 * (S // 64 + 1))
+    first = cache.add()
+    enc.text.extend(cache, [first], [ids[:S - 32]])
+
+    def instruction():  # 32 new tokens behind the rest of the prompt
+        seq = cache.fork(first, S - 32)
+        enc.text.extend(cache, [seq], [ids[S - 32:]])
+        cache.drop(seq)
+
+    timed("text_32_new_tokens", instruction)
     Sp = -(-S // 64) * 64
     D, F, L = tc.hidden_size, tc.intermediate_size, tc.num_hidden_layers
     kv = tc.num_key_value_heads * tc.head_dim
