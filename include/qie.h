@@ -398,7 +398,7 @@ int qie_silu_mul_bf16(const void* gu, int64_t ldg, int rows, int F, void* y, int
  *   (x, y) <- bf16(x cos - y sin), bf16(y cos + x sin),
  * (x, y) = elements (i, pairs + i), or (2i, 2i + 1) if interleaved; elements past 2 pairs pass
  * through. x: the first of `heads` heads, head_stride elements apart, of each of `rows` rows;
- * out: the same layout, x itself or memory apart from it. positions: int32 [axes], rows ldp apart;
+ * out: the same layout, x itself or memory apart from it. positions: int32 [axes][rows], ldp apart (0: shared);
  * turns: [pairs] (theta^(-i/n) / 2 pi for the usual ladder); axis: [pairs], clamped to the axes.
  * 4-byte aligned, even strides (16-byte rows and heads are the fast form); pairs <= 128. */
 int qie_rope_axes_bf16(const void* x, int64_t ldx, void* out, int64_t ldo, int rows, int heads, int head_dim,
@@ -429,7 +429,8 @@ int qie_attention_packed_bf16(const void* q, int64_t ldq, int64_t hsq, const voi
 
 /* Attention of the newest tokens of each sequence over a paged cache that holds them already: rows
  * [cu_seqlens[b], cu_seqlens[b + 1]) of q (one each if cu_seqlens is NULL) are the last n of the
- * kv_lens[b] cached tokens; query i sees keys j <= kv_lens[b] - n + i. Key j is slot j % page_size of
+ * kv_lens[b] cached tokens; query i sees keys j <= kv_lens[b] - n + i. Table rows are ld_table apart (0:
+ * shared). Key j is slot j % page_size of
  * page page_table[b][j / page_size] (a page outside the pool reads as zeros), pages as in
  * qie_rope_append_bf16. A row that sees no key is 0. Long rows are cut into chunks of keys whose
  * fp32 partials meet in `workspace` (>= qie_attention_paged_workspace bytes, 16-byte aligned, not

@@ -439,7 +439,7 @@ extern "C" int qie_attention_paged_bf16(const void* q, int64_t ldq, int64_t hsq,
                               kv_heads, head_dim, scale, out, ldo, hso));
   QIE_CHECK_ARG(page_table && kv_lens && (cu_seqlens || seqs == tokens) && num_pages > 0 && table_width > 0);
   QIE_CHECK_ARG(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0);
-  QIE_CHECK_ARG(page_stride >= 0 && page_stride % 8 == 0 && ld_table >= table_width);
+  QIE_CHECK_ARG(page_stride >= 0 && page_stride % 8 == 0 && (ld_table >= table_width || ld_table == 0));
   QIE_CHECK_ARG((int64_t)table_width * page_size <= INT32_MAX / 2);
   int64_t need = 0;
   const int rc = qie_attention_paged_workspace(tokens, seqs, heads, kv_heads, head_dim, table_width, page_size, &need);

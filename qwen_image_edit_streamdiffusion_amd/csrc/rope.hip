@@ -174,7 +174,7 @@ int launch_rope(RopeArgs& a, bool inter, hipStream_t s) {
 bool rope_common_ok(const void* x, const void* out, int rows, int head_dim, const int* positions, int64_t ldp,
                     int axes, const double* turns, const int* axis, int pairs) {
   return x && out && positions && turns && axis && rows >= 0 && head_dim > 0 && pairs > 0 && 2 * pairs <= head_dim &&
-         pairs <= kRopePairs && axes > 0 && ldp >= rows && (uintptr_t)x % 4 == 0 && (uintptr_t)out % 4 == 0 &&
+         pairs <= kRopePairs && axes > 0 && (ldp >= rows || ldp == 0) && (uintptr_t)x % 4 == 0 && (uintptr_t)out % 4 == 0 &&
          (uintptr_t)turns % 8 == 0;
 }
 

@@ -725,12 +725,13 @@ def _rows2(t: torch.Tensor, width: int, align: int, name: str) -> int:
 def _rope_args(T: int, head_dim: int, positions, turns, axis):
     pairs = turns.numel()
     st = positions.stride()
-    _chk(positions.dtype == torch.int32 and len(st) == 2 and positions.shape[1] == T and (T <= 1 or st[1] == 1),
-         "positions int32 [axes, rows]")
+    ldp = st[0] if len(st) == 2 and positions.shape[0] > 1 else T  # 0: one row for every axis (expand)
+    _chk(positions.dtype == torch.int32 and len(st) == 2 and positions.shape[0] > 0 and positions.shape[1] == T and
+         (T <= 1 or st[1] == 1) and (ldp == 0 or ldp >= T), "positions int32 [axes, rows]")
     _chk(turns.dtype == torch.float64 and turns.is_contiguous() and axis.dtype == torch.int32 and
          axis.is_contiguous() and axis.numel() == pairs, "turns float64 [pairs], axis int32 [pairs]")
     _chk(0 < 2 * pairs <= head_dim and pairs <= 128, "0 < 2 * pairs <= head_dim, pairs <= 128")
-    return (positions.data_ptr(), max(st[0], T), positions.shape[0], turns.data_ptr(), axis.data_ptr(), pairs)
+    return (positions.data_ptr(), ldp, positions.shape[0], turns.data_ptr(), axis.data_ptr(), pairs)
 
 
 def rope_axes(x: torch.Tensor, h0: int, nh: int, head_dim: int, positions: torch.Tensor, turns: torch.Tensor,
@@ -836,7 +837,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     [seqs + 1], ascending) of q [T, H, Dh] over the same rows of k, v [T, Hk, Dh], H a multiple of Hk;
     ``causal``: key j <= query i. Views of one projection's columns are fine. A query's result holds
     nothing of the keys it does not see. Rows outside every sequence are left as they were (``out``
-    given) or undefined."""
+    given, apart from k and v) or undefined."""
     dev = _same_dev(q, k, v, cu_seqlens, out)
     out, sc, ldq, hsq, ldo, hso = _seq_args(q, out, scale)
     T, H, Dh = q.shape
@@ -878,9 +879,10 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     N, Hk, P, ps, hs, ss = _pages(k_pages, v_pages, Dh)
     _chk(H % Hk == 0, "heads must be a multiple of kv_heads")
     tst = page_table.stride()
-    _chk(page_table.dtype == torch.int32 and len(tst) == 2 and page_table.numel() > 0 and tst[1] == 1,
-         "page_table int32 [seqs, width]")
+    _chk(page_table.dtype == torch.int32 and len(tst) == 2 and page_table.numel() > 0, "page_table int32 [seqs, width]")
     B, W = page_table.shape
+    ldt = tst[0] if B > 1 else W  # 0: one row for every sequence (expand)
+    _chk((W == 1 or tst[1] == 1) and (ldt == 0 or ldt >= W), "page_table: rows of consecutive entries")
     _chk(kv_lens.dtype == torch.int32 and kv_lens.dim() == 1 and kv_lens.numel() == B and kv_lens.is_contiguous(),
          "kv_lens int32 [seqs]")
     if cu_seqlens is None:
@@ -899,6 +901,6 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             have, wp = workspace.numel() * workspace.element_size(), workspace.data_ptr()
             _chk(have >= need and workspace.is_contiguous() and wp % 16 == 0, "workspace: contiguous, 16-byte aligned, large enough")
     _call_on("qie_attention_paged_bf16", dev, q.data_ptr(), ldq, hsq, k_pages.data_ptr(), v_pages.data_ptr(), N, P, ps,
-             hs, ss, page_table.data_ptr(), max(tst[0], W), W, kv_lens.data_ptr(),
+             hs, ss, page_table.data_ptr(), ldt, W, kv_lens.data_ptr(),
              None if cu_seqlens is None else cu_seqlens.data_ptr(), B, T, H, Hk, Dh, sc, out.data_ptr(), ldo, hso, wp, have)
     return out

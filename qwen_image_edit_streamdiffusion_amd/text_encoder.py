@@ -294,6 +294,7 @@ class QwenVLTextModel:
         if position_ids is None:
             position_ids = [torch.arange(cache.length(s), cache.length(s) + n).view(1, n).expand(3, n)
                             for s, n in zip(seqs, lens)]
+        self._check_positions(position_ids, lens)
         st = cache.step(seqs, lens)
         c = self.config
         H, Hk, Dh = c.num_attention_heads, c.num_key_value_heads, c.head_dim
@@ -307,16 +308,19 @@ class QwenVLTextModel:
 
         return list(self._rows(tokens, position_ids, lens, attend).split(lens))
 
+    def _check_positions(self, position_ids, lens):
+        if not self.layers:
+            raise RuntimeError("text encoder weights not loaded")
+        if len(position_ids) != len(lens) or any(tuple(p.shape) != (3, n) for p, n in zip(position_ids, lens)):
+            raise ValueError("positions [3, tokens] for each sequence")
+
     def _rows(self, prompts, position_ids, lens, attend) -> torch.Tensor:
         """The layers over the rows of all sequences, one behind the other; ``attend(layer, qkv, q, positions, out)``
         rotates the rows' heads and fills out [T, H, Dh]."""
         c, w, dev = self.config, self.w, self.device
-        if not self.layers:
-            raise RuntimeError("text encoder weights not loaded")
         D, H, Hk, Dh, F = c.hidden_size, c.num_attention_heads, c.num_key_value_heads, c.head_dim, c.intermediate_size
         T = sum(lens)
-        if len(position_ids) != len(lens) or any(tuple(p.shape) != (3, n) for p, n in zip(position_ids, lens)):
-            raise ValueError("positions [3, tokens] for each sequence")
+        self._check_positions(position_ids, lens)
         h = torch.empty(T, D, dtype=BF16, device=dev)
         if T == 0:
             return h

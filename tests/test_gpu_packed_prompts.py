@@ -79,6 +79,8 @@ def test_extend_over_the_cache_vs_transformers():
     got = te.extend(cache, [f], [other[70:]])[0]
     assert _rel(got, VL.text_forward(m, input_ids=other)[70:]) <= 2e-2
     more = torch.randint(0, 1000, (3,), generator=g)
+    with pytest.raises(ValueError):  # a refused call leaves the sequence as it was
+        te.extend(cache, [seqs[0]], [more], [torch.zeros(3, 4, dtype=torch.long)])
     got = te.extend(cache, [seqs[0]], [more])[0]
     assert _rel(got, VL.text_forward(m, input_ids=torch.cat([ids[0], more]))[150:]) <= 2e-2
 

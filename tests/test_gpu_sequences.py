@@ -217,7 +217,8 @@ def _split(xd, H, Hk, Dh):
 
 PACKED = [([1], 1, 1, 64), ([0, 5, 0, 64, 65, 0], 4, 2, 64), ([63, 1, 128, 200], 28, 4, 128), ([700], 6, 2, 128),
           ([33, 100], 16, 16, 80), ([129], 28, 1, 72), ([257, 64], 3, 3, 8), ([90, 400, 31], 16, 2, 96),
-          ([1] * 70 + [3], 7, 1, 40), ([1100, 2], 8, 8, 128), ([513, 1, 300], 20, 1, 128)]
+          ([1] * 70 + [3], 7, 1, 40), ([1100, 2], 8, 8, 128), ([513, 1, 300], 20, 1, 128), ([100], 28, 4, 128),
+          ([2600, 1500], 16, 2, 128), ([2600, 1500], 16, 2, 72), ([2600, 1500], 16, 2, 64)]  # the last: 256-row blocks
 
 
 @pytest.mark.parametrize("causal", [True, False])
@@ -246,12 +247,12 @@ def test_attention_packed_long_and_large_logits():
     _check(ops.attention_packed(qd, kd, vd, _cu(lens).to(DEV), scale=0.01), want, tol)
 
 
-@pytest.mark.parametrize("lens", [[70, 130], [600, 900]])
-def test_attention_packed_rows_outside_and_nonfinite_neighbours(lens):
+@pytest.mark.parametrize("lens,H,Hk", [([70, 130], 6, 2), ([600, 900], 6, 2), ([20, 40], 6, 2), ([150, 2500], 22, 2)])
+def test_attention_packed_rows_outside_and_nonfinite_neighbours(lens, H, Hk):
     """Rows behind the last sequence stay as they were; infinities and NaN of another sequence, behind
     the last one, or of a later key do not reach a query that does not see them; one that it sees does."""
     ops = _ops()
-    H, Hk, Dh = 6, 2, 128
+    Dh = 128
     T = sum(lens) + 40
     g = _gen(9)
     x, q, k, v = _qkv(g, T, H, Hk, Dh)
@@ -330,7 +331,10 @@ PAGED = [([1], [1], 1, 1, 64, 16, "heads"), ([1, 1, 1], [5, 700, 64], 28, 4, 128
          ([1] * 5, [0, 513, 1, 2000, 512], 7, 1, 128, 16, "rows"), ([41], [309], 28, 4, 128, 64, "rows"),
          ([3, 0, 9], [2, 50, 1300], 6, 2, 80, 32, "heads"), ([300, 17], [300, 1100], 4, 4, 128, 128, "heads"),
          ([64, 130], [64, 5000], 8, 2, 96, 16, "rows"), ([700], [1500], 14, 2, 72, 1024, "heads"),
-         ([2] * 67, [40] * 66 + [3000], 20, 1, 128, 64, "heads"), ([600, 900], [5000, 2500], 28, 4, 128, 64, "heads")]
+         ([2] * 67, [40] * 66 + [3000], 20, 1, 128, 64, "heads"), ([600, 900], [5000, 2500], 28, 4, 128, 64, "heads"),
+         ([300, 200], [300, 400], 28, 4, 128, 16, "rows"), ([300, 200], [300, 400], 28, 4, 64, 64, "heads"),
+         ([8] * 20, [8] * 19 + [3000], 28, 4, 128, 16, "heads"), ([700, 900], [700, 3000], 16, 2, 80, 32, "rows"),
+         ([30], [400], 40, 1, 128, 64, "heads"), ([2500], [2500], 16, 2, 64, 16, "heads")]
 
 
 @pytest.mark.parametrize("new,kv,H,Hk,Dh,P,layout", PAGED)
@@ -346,19 +350,63 @@ def test_attention_paged(new, kv, H, Hk, Dh, P, layout):
         assert torch.equal(ops.attention_paged(q.to(DEV), kp, vp, table.to(DEV), kvl), got)
 
 
-def test_attention_paged_rows_do_not_depend_on_the_batch():
-    """The same sequence alone and among others: bitwise the same rows (the cuts go by its own length)."""
+@pytest.mark.parametrize("new,kv", [([1, 1, 1], [900, 2600, 30]), ([40, 5, 9], [900, 2600, 30]), ([300, 20, 700], [900, 2600, 800])])
+def test_attention_paged_rows_do_not_depend_on_other_sequences(new, kv):
+    """In calls of one shape a row's bits do not depend on the other sequences' lengths and values."""
     ops = _ops()
-    new, kv, H, Hk, Dh, P = [1, 5, 1], [900, 2600, 30], 28, 4, 128, 64
+    H, Hk, Dh, P = 28, 4, 128, 64
     q, ks, vs, kp, vp, table = _paged(_gen(1), new, kv, H, Hk, Dh, P)
     i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
-    qd, td = q.to(DEV), table.to(DEV)
-    got = ops.attention_paged(qd, kp, vp, td, i32(kv), cu_seqlens=_cu(new).to(DEV))
-    at = 0
-    for b, n in enumerate(new):
-        one = ops.attention_paged(qd[at:at + n], kp, vp, td[b:b + 1], i32(kv[b:b + 1]), cu_seqlens=_cu([n]).to(DEV))
-        assert torch.equal(one, got[at:at + n])
-        at += n
+    qd, td, cu = q.to(DEV), table.to(DEV), _cu(new).to(DEV)
+    got = ops.attention_paged(qd, kp, vp, td, i32(kv), cu_seqlens=cu)
+    q2 = qd.clone()
+    q2[:new[0]], q2[new[0] + new[1]:] = 3.0, -1.0
+    other = ops.attention_paged(q2, kp, vp, td, i32([new[0], kv[1], new[2]]), cu_seqlens=cu)
+    mid = slice(new[0], new[0] + new[1])
+    assert torch.equal(other[mid], got[mid]) and not torch.equal(other[:new[0]], got[:new[0]])
+
+
+@pytest.mark.parametrize("new,kv,H,Hk", [(60, 100, 28, 4), (7, 2000, 6, 1), (9, 2600, 28, 4), (400, 450, 28, 4), (30, 3000, 40, 1),
+                                         (1200, 3000, 28, 4)])
+def test_attention_paged_nonfinite_later_keys(new, kv, H, Hk):
+    """Infinities and NaN of a later key of the same chunk do not reach the queries before it."""
+    ops = _ops()
+    Dh, P = 128, 32
+    q, ks, vs, kp, vp, table = _paged(_gen(kv), [new], [kv], H, Hk, Dh, P)
+    want, tol = paged_ref(q, ks, vs, [new], [kv])
+    bad = kv - 3  # query new - 3 and later ones see it
+    page, slot = int(table[0, bad // P]), bad % P
+    vp[page, :, slot, 5], vp[page, :, slot, 7] = float("nan"), float("-inf")
+    nxt = kv - 2
+    kp[int(table[0, nxt // P]), :, nxt % P] = float("inf")
+    got = ops.attention_paged(q.to(DEV), kp, vp, table.to(DEV), torch.tensor([kv], dtype=torch.int32, device=DEV),
+                              cu_seqlens=_cu([new]).to(DEV)).cpu()
+    _check(got[:new - 3], want[:new - 3], tol[:new - 3])
+    keep = [d for d in range(Dh) if d not in (5, 7)]
+    _check(got[new - 3][:, keep], want[new - 3][:, keep], tol[new - 3][:, keep])
+    assert torch.isnan(got[new - 3, :, 5]).all() and (got[new - 3, :, 7] == float("-inf")).all()
+    assert not torch.isfinite(got[new - 2:]).all(-1).any()
+
+
+def test_shared_rows_of_positions_and_tables():
+    """expand()ed positions (one row for every axis) and tables (one for every sequence)."""
+    ops = _ops()
+    turns, axis, axes, _ = _plan("sections")
+    d = lambda t: t.to(DEV)  # noqa: E731
+    x = _randn(_gen(1), 33, 256)
+    row = torch.arange(33, dtype=torch.int32).view(1, 33)
+    a = ops.rope_axes(d(x), 0, 2, 128, d(row).expand(3, 33), d(turns), d(axis))
+    b = ops.rope_axes(d(x), 0, 2, 128, d(row.repeat(3, 1)), d(turns), d(axis))
+    assert torch.equal(a, b)
+    q, ks, vs, kp, vp, table = _paged(_gen(2), [1], [100], 4, 2, 128, 16)
+    q3 = _randn(_gen(3), 3, 4, 128)
+    lens = [100, 57, 3]
+    got = ops.attention_paged(d(q3), kp, vp, d(table).expand(3, -1), torch.tensor(lens, dtype=torch.int32, device=DEV))
+    for b, n in enumerate(lens):
+        want, tol = paged_ref(q3[b:b + 1], [ks[0][:n]], [vs[0][:n]], [1], [n])
+        _check(got[b:b + 1], want, tol)
+    with pytest.raises(ValueError):  # rows that overlap
+        ops.rope_axes(d(x), 0, 2, 128, torch.zeros(40, dtype=torch.int32, device=DEV).as_strided((3, 33), (2, 1)), d(turns), d(axis))
 
 
 def test_attention_paged_bad_pages_read_as_zeros():

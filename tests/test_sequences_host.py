@@ -53,7 +53,7 @@ def test_entry_points_refuse_on_the_host(lib):
                dict(pairs=0), dict(pairs=65), dict(pairs=129, dh=512, hs=512), dict(axes=0), dict(ldp=3), dict(hs=127),
                dict(hs=64), dict(ldx=511), dict(ldx=510), dict(ldo=256), dict(x=18), dict(turns=20)):
         assert rope(**kw) == -1, kw
-    assert rope(rows=0, ldp=0) == 0  # nothing to do
+    assert rope(rows=0) == 0  # nothing to do
 
     ok2 = dict(x=16, ldx=768, out=16, ldo=512, rows=4, H=4, Hk=1, dh=128, pos=16, ldp=4, axes=3, turns=16, axis=16, pairs=64,
                k=16, v=16, N=2, P=16, ps=2048, hs=2048, ss=128, slots=16)
