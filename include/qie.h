@@ -421,7 +421,7 @@ int qie_rope_append_bf16(const void* qkv, int64_t ldx, void* q_out, int64_t ldo,
  * reads kv head h / (heads / kv_heads)); causal: key j <= query i. fp32 softmax, P rounded to bf16
  * for P.V. What a query does not see does not reach it, infinities and NaN included. Rows outside
  * every sequence are left as they were. Strides in elements, multiples of 8; head_dim % 8 == 0,
- * <= 128; scale > 0. */
+ * <= 128; 0 < scale <= 65536; out: q itself or memory apart from it (in the next one as well). */
 int qie_attention_packed_bf16(const void* q, int64_t ldq, int64_t hsq, const void* k, const void* v, int64_t ldk,
                               int64_t hsk, const int* cu_seqlens, int seqs, int tokens, int heads, int kv_heads,
                               int head_dim, int causal, float scale, void* out, int64_t ldo, int64_t hso,
@@ -429,10 +429,9 @@ int qie_attention_packed_bf16(const void* q, int64_t ldq, int64_t hsq, const voi
 
 /* Attention of the newest tokens of each sequence over a paged cache that holds them already: rows
  * [cu_seqlens[b], cu_seqlens[b + 1]) of q (one each if cu_seqlens is NULL) are the last n of the
- * kv_lens[b] cached tokens; query i sees keys j <= kv_lens[b] - n + i. Table rows are ld_table apart (0:
- * shared). Key j is slot j % page_size of
- * page page_table[b][j / page_size] (a page outside the pool reads as zeros), pages as in
- * qie_rope_append_bf16. A row that sees no key is 0. Long rows are cut into chunks of keys whose
+ * kv_lens[b] cached tokens; query i sees keys j <= kv_lens[b] - n + i. Key j is slot
+ * j % page_size of page page_table[b][j / page_size] (a page outside the pool reads as zeros; table rows
+ * ld_table apart, 0: shared), pages as in qie_rope_append_bf16. A row that sees no key is 0. Long rows are cut into chunks of keys whose
  * fp32 partials meet in `workspace` (>= qie_attention_paged_workspace bytes, 16-byte aligned, not
  * shared with a call that may run at the same time; 0 bytes, and NULL is fine, for tables of up to
  * 1024 tokens). The cuts go by the call's counts, never by the values of lengths or tables: in calls

@@ -109,6 +109,7 @@ __device__ __forceinline__ bool find_item(const SeqArgs& a, int idx, Item& it) {
       it.n = __builtin_amdgcn_readlane(n, l);
       it.kv = __builtin_amdgcn_readlane(kv, l);
       const int j = idx - __builtin_amdgcn_readlane(pre - cnt, l);
+      if (j < 0 || j >= __builtin_amdgcn_readlane(cnt, l)) return false;  // offsets that overlap: sums past 32 bits
       it.nch = a.ct ? max(1, (it.kv + a.ct * kKB - 1) / (a.ct * kKB)) : 1;
       const int nblk = (it.n * a.G + BM - 1) / BM;
       it.ch = j / nblk;               // neighbours read the same keys

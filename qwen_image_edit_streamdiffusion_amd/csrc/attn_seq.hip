@@ -392,7 +392,7 @@ bool seq_common_ok(const void* q, int64_t ldq, int64_t hsq, const void* k, const
                    int seqs, int tokens, int heads, int kv_heads, int head_dim, float scale, const void* out,
                    int64_t ldo, int64_t hso) {
   if (!(q && k && v && out && seqs > 0 && tokens >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0)) return false;
-  if (!(head_dim > 0 && head_dim <= 128 && head_dim % 8 == 0 && scale > 0.f && scale < INFINITY)) return false;
+  if (!(head_dim > 0 && head_dim <= 128 && head_dim % 8 == 0 && scale > 0.f && scale <= 65536.f)) return false;
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16 != 0) return false;
   if ((ldq | hsq | ldk | hsk | ldo | hso) % 8 != 0) return false;
   if (ldq < 0 || hsq < 0 || ldk < head_dim || ldk > (1 << 23) || hsk < 0 || ldo < head_dim || hso < head_dim) return false;

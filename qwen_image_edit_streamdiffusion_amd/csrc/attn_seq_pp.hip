@@ -282,7 +282,8 @@ __global__ void __launch_bounds__(512) attn_seq_pp_kernel(SeqArgs a) {
     __builtin_amdgcn_s_waitcnt(0);  // q as well: from here on the counter is the tiles'
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     if (grp == 1) asm volatile("s_barrier" ::: "memory");
-    auto mend = [&]() { asm volatile("s_barrier" ::: "memory"); };
+    // asm products are not padded: the softmax may read the last ones' results (S on the first tile) 16 cycles on
+    auto mend = [&]() { asm volatile("s_nop 15\n\ts_barrier" ::: "memory"); };
     first(I0{}, t0, t0);
     products(I0{}, IQ{}, IQ{}, t0, t0);
     mend();

@@ -820,7 +820,7 @@ def _seq_args(q: torch.Tensor, out, scale):
     H, Dh = q.shape[1:]
     _chk(H > 0 and 0 < Dh <= 128 and Dh % 8 == 0, "head_dim: a multiple of 8, <= 128")
     sc = 1.0 / math.sqrt(Dh) if scale is None else float(scale)
-    _chk(0.0 < sc < math.inf, "scale must be positive and finite")
+    _chk(0.0 < sc <= 65536.0, "scale: positive, at most 65536")
     if out is None:
         out = torch.empty(q.shape, dtype=BF16, device=q.device)
         return out, sc, ldq, hsq, H * Dh, Dh
@@ -837,7 +837,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     [seqs + 1], ascending) of q [T, H, Dh] over the same rows of k, v [T, Hk, Dh], H a multiple of Hk;
     ``causal``: key j <= query i. Views of one projection's columns are fine. A query's result holds
     nothing of the keys it does not see. Rows outside every sequence are left as they were (``out``
-    given, apart from k and v) or undefined."""
+    given: q itself or memory apart from q, k and v) or undefined."""
     dev = _same_dev(q, k, v, cu_seqlens, out)
     out, sc, ldq, hsq, ldo, hso = _seq_args(q, out, scale)
     T, H, Dh = q.shape
@@ -871,7 +871,7 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     cu_seqlens) are the last n of the kv_lens[b] tokens (device int32 [seqs]); query i sees keys
     j <= kv_lens[b] - n + i, 0 where it sees none. Key j: slot j % page_size of page
     page_table[b, j // page_size] (device int32 [seqs, width]; a page outside the pool reads as zeros)
-    of k_pages, v_pages [pages, Hk, page_size, Dh]. ``workspace`` (>= attention_paged_workspace_bytes,
+    of k_pages, v_pages [pages, Hk, page_size, Dh]. ``out``: q itself or memory apart from it. ``workspace`` (>= attention_paged_workspace_bytes,
     not shared with a call that may run at the same time) is taken from torch's allocator if not given."""
     dev = _same_dev(q, k_pages, v_pages, page_table, kv_lens, cu_seqlens, out, workspace)
     out, sc, ldq, hsq, ldo, hso = _seq_args(q, out, scale)

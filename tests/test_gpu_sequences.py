@@ -563,6 +563,41 @@ def test_other_stream():
     assert torch.equal(got, ref)
 
 
+@pytest.mark.parametrize("new,kv", [([1, 1, 1], [3000, 5, 700]), ([40, 3, 60], [3000, 300, 60]), ([700, 5, 900], [3000, 300, 900])])
+def test_two_streams_and_in_place(new, kv):
+    """Two calls at once, each with its own workspace, and a call whose out is q: bitwise the call alone."""
+    ops = _ops()
+    H, Hk, Dh, P = 28, 4, 128, 64
+    q, ks, vs, kp, vp, table = _paged(_gen(21), new, kv, H, Hk, Dh, P)
+    qd, td, cu, lens = q.to(DEV), table.to(DEV), _cu(new).to(DEV), torch.tensor(kv, dtype=torch.int32, device=DEV)
+    q2 = -qd
+    run = lambda x, **kw: ops.attention_paged(x, kp, vp, td, lens, cu_seqlens=cu, **kw)  # noqa: E731
+    want, want2 = run(qd), run(q2)
+    n = ops.attention_paged_workspace_bytes(len(q), len(kv), H, Hk, Dh, table.shape[1], P)
+    ws = [torch.empty(max(n, 16), dtype=torch.uint8, device=DEV) for _ in range(2)]
+    outs = [torch.empty_like(qd) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, x, o, w in zip(streams, (qd, q2), outs, ws):
+            with torch.cuda.stream(s):
+                run(x, out=o, workspace=w)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], want2)
+    assert run(q2, out=q2) is q2 and torch.equal(q2, want2)
+
+
+@pytest.mark.parametrize("lens", [[40, 30], [300, 500, 9], [2600, 1500]])
+def test_packed_in_place(lens):
+    ops = _ops()
+    x, q, k, v = _qkv(_gen(22), sum(lens), 16, 2, 128)
+    xd = x.to(DEV)
+    qd, kd, vd = _split(xd, 16, 2, 128)
+    want = ops.attention_packed(qd, kd, vd, _cu(lens).to(DEV))
+    ops.attention_packed(qd, kd, vd, _cu(lens).to(DEV), out=qd)
+    assert torch.equal(qd, want) and torch.equal(kd.cpu(), k) and torch.equal(vd.cpu(), v)
+
+
 def test_empty_calls():
     ops = _ops()
     z = lambda *s, dt=BF16: torch.zeros(*s, dtype=dt, device=DEV)  # noqa: E731

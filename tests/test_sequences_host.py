@@ -75,7 +75,7 @@ def test_entry_points_refuse_on_the_host(lib):
         return lib.qie_attention_packed_bf16(a["q"], a["ldq"], a["hsq"], a["k"], a["v"], a["ldk"], a["hsk"], a["cu"], a["B"],
                                              a["T"], a["H"], a["Hk"], a["dh"], 1, a["sc"], a["out"], a["ldo"], a["hso"], None)
     refused = (dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(B=0), dict(T=-1), dict(H=0), dict(Hk=0),
-               dict(Hk=3), dict(dh=0), dict(dh=136), dict(dh=60), dict(sc=0.0), dict(sc=-1.0), dict(sc=math.inf),
+               dict(Hk=3), dict(dh=0), dict(dh=136), dict(dh=60), dict(sc=0.0), dict(sc=-1.0), dict(sc=math.inf), dict(sc=65537.0),
                dict(sc=math.nan), dict(q=24), dict(ldq=516), dict(ldk=64), dict(hso=64), dict(T=1 << 30))
     for kw in refused + (dict(cu=None),):
         assert packed(**kw) == -1, kw
