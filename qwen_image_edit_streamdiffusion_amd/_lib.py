@@ -124,3 +124,17 @@ def call(name: str, *args) -> None:
     if rc != 0:
         msg = lib.qie_strerror(rc).decode()
         raise QieError(f"{name} failed ({rc}): {msg}")
+
+
+def load_calls():
+    """The native module of the operators on sequences (csrc/seq_bind.cpp), bound to the loaded libqie."""
+    lib = load()
+    try:
+        from . import _seq
+    except ImportError as e:
+        raise QieError(f"_seq.so, built beside libqie.so, is required ({e}). Build it with "
+                       "`python -c 'import __graft_entry__ as g; g.build()'`.") from e
+    at = lambda name: ctypes.cast(getattr(lib, name), c_void_p).value  # noqa: E731
+    _seq.bind(QieError, *(at(n) for n in ("qie_rope_axes_bf16", "qie_rope_append_bf16", "qie_attention_packed_bf16",
+                                          "qie_attention_paged_bf16", "qie_attention_paged_workspace", "qie_strerror")))
+    return _seq

@@ -694,44 +694,17 @@ def silu_mul(gu: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tens
 
 
 # ---------------------------------------------------------------------------- sequences and their cache
-# Small calls are bound by the host: strides come from one stride() each, the stream from the raw getter.
-def _call_on(name: str, dev: int, *args) -> None:
-    """Launch on the current stream of device ``dev``, the operands', which need not be the current one."""
-    if dev == torch._C._cuda_getDevice():
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+# Small calls are bound by the host: checks, strides, the stream of the operands' device and the call of
+# libqie are one native step (csrc/seq_bind.cpp).
+_seq_calls = None
 
 
-def _same_dev(*ts) -> int:
-    """The one device of the tensors."""
-    dev = ts[0].get_device()
-    for t in ts:
-        if dev < 0 or (t is not None and t.get_device() != dev):
-            raise ValueError("libqie ops need tensors of one device")
-    return dev
-
-
-def _rows2(t: torch.Tensor, width: int, align: int, name: str) -> int:
-    """Row stride of a bf16 row-major view [T, >= width]; of a single row, whose stride says nothing, its width."""
-    st = t.stride()
-    ld = st[0] if t.shape[0] > 1 else -(-width // 8) * 8
-    if t.dtype != BF16 or len(st) != 2 or st[1] != 1 or t.shape[1] < width or ld % align or t.data_ptr() % (2 * align):
-        raise ValueError(f"{name}: bf16 row-major [rows, >= {width}], rows aligned to {2 * align} bytes")
-    return ld
-
-
-def _rope_args(T: int, head_dim: int, positions, turns, axis):
-    pairs = turns.numel()
-    st = positions.stride()
-    ldp = st[0] if len(st) == 2 and positions.shape[0] > 1 else T  # 0: one row for every axis (expand)
-    _chk(positions.dtype == torch.int32 and len(st) == 2 and positions.shape[0] > 0 and positions.shape[1] == T and
-         (T <= 1 or st[1] == 1) and (ldp == 0 or ldp >= T), "positions int32 [axes, rows]")
-    _chk(turns.dtype == torch.float64 and turns.is_contiguous() and axis.dtype == torch.int32 and
-         axis.is_contiguous() and axis.numel() == pairs, "turns float64 [pairs], axis int32 [pairs]")
-    _chk(0 < 2 * pairs <= head_dim and pairs <= 128, "0 < 2 * pairs <= head_dim, pairs <= 128")
-    return (positions.data_ptr(), ldp, positions.shape[0], turns.data_ptr(), axis.data_ptr(), pairs)
+def _seq():
+    """The native module, its entry points bound to the loaded libqie."""
+    global _seq_calls
+    if _seq_calls is None:
+        _seq_calls = _lib.load_calls()
+    return _seq_calls
 
 
 def rope_axes(x: torch.Tensor, h0: int, nh: int, head_dim: int, positions: torch.Tensor, turns: torch.Tensor,
@@ -742,37 +715,8 @@ def rope_axes(x: torch.Tensor, h0: int, nh: int, head_dim: int, positions: torch
     (``rope.section_turns`` / ``rope.axes_turns`` make turns and axis). Pairs are half a rotary width
     apart, or neighbours if ``interleaved``. In place, or into ``out`` [T, >= nh heads], whose first
     head is head h0 and which does not overlap x; one rounding, angles in 64 bits."""
-    dev = _same_dev(x, positions, turns, axis, out)
-    hs = head_dim if head_stride is None else head_stride
-    _chk(h0 >= 0 and nh >= 1 and hs >= head_dim and hs % 2 == 0, "heads, an even stride apart")
-    width = (nh - 1) * hs + head_dim
-    ldx = _rows2(x, h0 * hs + width, 2, "x")
-    T = x.shape[0]
-    rope = _rope_args(T, head_dim, positions, turns, axis)
-    xp = x.data_ptr() + 2 * h0 * hs
-    if out is None:
-        op, ldo = xp, ldx
-    else:
-        ldo = _rows2(out, width, 2, "out")
-        _chk(out.shape[0] == T, "out [T, heads]")
-        op = out.data_ptr()
-    if T:
-        _call_on("qie_rope_axes_bf16", dev, xp, ldx, op, ldo, T, nh, head_dim, hs, *rope, int(interleaved))
-    return x if out is None else out
-
-
-def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, head_dim: int):
-    """Checks of a cache's pages [pages, kv_heads, page_size, head_dim] -> their strides."""
-    st = k_pages.stride()
-    _chk(k_pages.dtype == BF16 and v_pages.dtype == BF16 and len(st) == 4 and k_pages.shape == v_pages.shape and
-         st == v_pages.stride(), "k_pages / v_pages: bf16 [pages, kv_heads, page_size, head_dim], same strides")
-    N, Hk, P, Dh = k_pages.shape
-    ps, hs, ss, one = st
-    _chk(N > 0 and Hk > 0 and Dh == head_dim and Dh % 8 == 0 and one == 1, "pages: rows of head_dim, a multiple of 8")
-    _chk(16 <= P <= 1024 and P & (P - 1) == 0, "page_size: a power of two in [16, 1024]")
-    _chk((ps | hs | ss) % 8 == 0 and ss >= Dh and (N == 1 or ps >= Dh) and (Hk == 1 or hs >= Dh) and
-         (k_pages.data_ptr() | v_pages.data_ptr()) % 16 == 0, "pages: 16-byte aligned rows that do not overlap")
-    return N, Hk, P, ps, hs, ss
+    return (_seq_calls or _seq()).rope_axes(x, positions, turns, axis, out, h0, nh, head_dim,
+                                            head_dim if head_stride is None else head_stride, interleaved)
 
 
 def rope_append(qkv: torch.Tensor, heads: int, kv_heads: int, head_dim: int, positions: torch.Tensor,
@@ -782,52 +726,8 @@ def rope_append(qkv: torch.Tensor, heads: int, kv_heads: int, head_dim: int, pos
     cache: the rotated q goes to ``out`` [T, heads * head_dim] (default: in place), the rotated k and
     v of row t to slot ``slots[t] % page_size`` of page ``slots[t] // page_size`` (int64; < 0 or past
     the pool: not stored; the slots of one call must be distinct). Returns the q rows."""
-    dev = _same_dev(qkv, positions, turns, axis, k_pages, v_pages, slots, out)
-    _chk(heads > 0 and kv_heads > 0, "heads")
-    ldx = _rows2(qkv, (heads + 2 * kv_heads) * head_dim, 8, "qkv")
-    T = qkv.shape[0]
-    N, Hk, P, ps, hs, ss = _pages(k_pages, v_pages, head_dim)
-    _chk(Hk == kv_heads, "pages of another number of kv heads")
-    _chk(slots.dtype == torch.int64 and slots.dim() == 1 and slots.numel() == T and slots.is_contiguous(), "slots int64 [T]")
-    rope = _rope_args(T, head_dim, positions, turns, axis)
-    if out is None:
-        out = qkv[:, :heads * head_dim]
-        ldo = ldx
-    else:
-        ldo = _rows2(out, heads * head_dim, 8, "out")
-        _chk(tuple(out.shape) == (T, heads * head_dim), "out [T, heads * head_dim]")
-    if T:
-        _call_on("qie_rope_append_bf16", dev, qkv.data_ptr(), ldx, out.data_ptr(), ldo, T, heads, kv_heads, head_dim,
-                 *rope, int(interleaved), k_pages.data_ptr(), v_pages.data_ptr(), N, P, ps, hs, ss, slots.data_ptr())
-    return out
-
-
-def _heads3(t: torch.Tensor, name: str):
-    """(row stride, head stride) of a [T, heads, head_dim] view with 16-byte aligned heads."""
-    st = t.stride()
-    if len(st) != 3:
-        raise ValueError(name + ": [T, heads, head_dim]")
-    T, H, Dh = t.shape
-    ld, hs = st[0] if T > 1 else H * Dh, st[1] if H > 1 else Dh
-    if t.dtype != BF16 or st[2] != 1 or (ld | hs) % 8 or t.data_ptr() % 16:
-        raise ValueError(name + ": bf16 [T, heads, head_dim], 16-byte aligned heads")
-    return ld, hs
-
-
-def _seq_args(q: torch.Tensor, out, scale):
-    """Strides of q and of out (made here if not given), the scale."""
-    ldq, hsq = _heads3(q, "q")
-    H, Dh = q.shape[1:]
-    _chk(H > 0 and 0 < Dh <= 128 and Dh % 8 == 0, "head_dim: a multiple of 8, <= 128")
-    sc = 1.0 / math.sqrt(Dh) if scale is None else float(scale)
-    _chk(0.0 < sc <= 65536.0, "scale: positive, at most 65536")
-    if out is None:
-        out = torch.empty(q.shape, dtype=BF16, device=q.device)
-        return out, sc, ldq, hsq, H * Dh, Dh
-    _chk(out.shape == q.shape, "out [T, heads, head_dim]")
-    ldo, hso = _heads3(out, "out")
-    _chk(ldo >= Dh and hso >= Dh, "out: rows that do not overlap")
-    return out, sc, ldq, hsq, ldo, hso
+    return (_seq_calls or _seq()).rope_append(qkv, positions, turns, axis, k_pages, v_pages, slots, out, heads, kv_heads,
+                                              head_dim, interleaved)
 
 
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -838,21 +738,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     ``causal``: key j <= query i. Views of one projection's columns are fine. A query's result holds
     nothing of the keys it does not see. Rows outside every sequence are left as they were (``out``
     given: q itself or memory apart from q, k and v) or undefined."""
-    dev = _same_dev(q, k, v, cu_seqlens, out)
-    out, sc, ldq, hsq, ldo, hso = _seq_args(q, out, scale)
-    T, H, Dh = q.shape
-    kst = _heads3(k, "k")
-    Hk = k.shape[1]
-    _chk(k.shape == v.shape and k.shape[0] == T and k.shape[2] == Dh and Hk > 0 and H % Hk == 0,
-         "k, v [T, kv_heads, head_dim], heads a multiple of kv_heads")
-    _chk(kst == _heads3(v, "v") and kst[0] >= Dh, "k and v: the same strides, rows that do not overlap")
-    B = cu_seqlens.numel() - 1
-    _chk(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and B >= 1 and cu_seqlens.is_contiguous(),
-         "cu_seqlens int32 [seqs + 1]")
-    if T:
-        _call_on("qie_attention_packed_bf16", dev, q.data_ptr(), ldq, hsq, k.data_ptr(), v.data_ptr(), kst[0], kst[1],
-                 cu_seqlens.data_ptr(), B, T, H, Hk, Dh, int(causal), sc, out.data_ptr(), ldo, hso)
-    return out
+    return (_seq_calls or _seq()).attention_packed(q, k, v, cu_seqlens, out, causal, scale)
 
 
 def attention_paged_workspace_bytes(tokens: int, seqs: int, heads: int, kv_heads: int, head_dim: int,
@@ -871,36 +757,7 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     cu_seqlens) are the last n of the kv_lens[b] tokens (device int32 [seqs]); query i sees keys
     j <= kv_lens[b] - n + i, 0 where it sees none. Key j: slot j % page_size of page
     page_table[b, j // page_size] (device int32 [seqs, width]; a page outside the pool reads as zeros)
-    of k_pages, v_pages [pages, Hk, page_size, Dh]. ``out``: q itself or memory apart from it. ``workspace`` (>= attention_paged_workspace_bytes,
-    not shared with a call that may run at the same time) is taken from torch's allocator if not given."""
-    dev = _same_dev(q, k_pages, v_pages, page_table, kv_lens, cu_seqlens, out, workspace)
-    out, sc, ldq, hsq, ldo, hso = _seq_args(q, out, scale)
-    T, H, Dh = q.shape
-    N, Hk, P, ps, hs, ss = _pages(k_pages, v_pages, Dh)
-    _chk(H % Hk == 0, "heads must be a multiple of kv_heads")
-    tst = page_table.stride()
-    _chk(page_table.dtype == torch.int32 and len(tst) == 2 and page_table.numel() > 0, "page_table int32 [seqs, width]")
-    B, W = page_table.shape
-    ldt = tst[0] if B > 1 else W  # 0: one row for every sequence (expand)
-    _chk((W == 1 or tst[1] == 1) and (ldt == 0 or ldt >= W), "page_table: rows of consecutive entries")
-    _chk(kv_lens.dtype == torch.int32 and kv_lens.dim() == 1 and kv_lens.numel() == B and kv_lens.is_contiguous(),
-         "kv_lens int32 [seqs]")
-    if cu_seqlens is None:
-        _chk(T == B, "one q row a sequence without cu_seqlens")
-    else:
-        _chk(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.numel() == B + 1 and
-             cu_seqlens.is_contiguous(), "cu_seqlens int32 [seqs + 1]")
-    if T == 0:
-        return out
-    have = wp = 0
-    if W * P > 1024:
-        need = attention_paged_workspace_bytes(T, B, H, Hk, Dh, W, P)
-        if need and workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        if workspace is not None:
-            have, wp = workspace.numel() * workspace.element_size(), workspace.data_ptr()
-            _chk(have >= need and workspace.is_contiguous() and wp % 16 == 0, "workspace: contiguous, 16-byte aligned, large enough")
-    _call_on("qie_attention_paged_bf16", dev, q.data_ptr(), ldq, hsq, k_pages.data_ptr(), v_pages.data_ptr(), N, P, ps,
-             hs, ss, page_table.data_ptr(), ldt, W, kv_lens.data_ptr(),
-             None if cu_seqlens is None else cu_seqlens.data_ptr(), B, T, H, Hk, Dh, sc, out.data_ptr(), ldo, hso, wp, have)
-    return out
+    of k_pages, v_pages [pages, Hk, page_size, Dh]. ``out``: q itself or memory apart from it.
+    ``workspace`` (>= attention_paged_workspace_bytes, not shared with a call that may run at the same
+    time) is taken from torch's allocator if not given."""
+    return (_seq_calls or _seq()).attention_paged(q, k_pages, v_pages, page_table, kv_lens, cu_seqlens, out, workspace, scale)

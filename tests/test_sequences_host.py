@@ -98,6 +98,25 @@ def test_entry_points_refuse_on_the_host(lib):
     assert lib.qie_attention_paged_workspace(4, 1, 4, 1, 128, 4096, 16, None) == -1
 
 
+def test_calls_refuse_host_tensors_and_other_objects():
+    """The native calls take device tensors only, and say which argument is none."""
+    from qwen_image_edit_streamdiffusion_amd import ops
+    from qwen_image_edit_streamdiffusion_amd.rope import section_turns
+    turns, axis = section_turns((16, 24, 24), 1e6, "cpu")
+    x = torch.zeros(4, 768, dtype=torch.bfloat16)
+    q, pages = x[:, :512].unflatten(1, (4, 128)), torch.zeros(2, 1, 16, 128, dtype=torch.bfloat16)
+    pos, cu = torch.zeros(3, 4, dtype=torch.int32), torch.tensor([0, 4], dtype=torch.int32)
+    for fn in (lambda: ops.rope_axes(x, 0, 4, 128, pos, turns, axis), lambda: ops.attention_packed(q, q, q, cu),
+               lambda: ops.rope_append(x, 4, 1, 128, pos, turns, axis, pages, pages, torch.arange(4)),
+               lambda: ops.attention_paged(q, pages, pages, pos, cu)):
+        with pytest.raises(ValueError):
+            fn()
+    for fn in (lambda: ops.rope_axes([1.0], 0, 4, 128, pos, turns, axis), lambda: ops.attention_packed(None, q, q, cu),
+               lambda: ops.attention_paged(q.numpy, pages, pages, pos, cu)):
+        with pytest.raises(TypeError):
+            fn()
+
+
 # ---------------------------------------------------------------------------- the cache's pages
 def _cache(pages=8):
     from qwen_image_edit_streamdiffusion_amd.kv_cache import PagedKVCache
