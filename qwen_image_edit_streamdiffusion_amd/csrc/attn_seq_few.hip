@@ -28,14 +28,7 @@ __global__ void __launch_bounds__(64 * NW) attn_seq_few_kernel(SeqArgs a) {
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
   const int g = lane >> 4, ql = lane & 15;
   const int rows = it.n * a.G, row0 = it.blk * BM;
-  const int off = it.kv - it.n;
-  const int last = (min(rows, row0 + BM) - 1) / a.G;
-  const int most = a.causal ? min(it.kv, max(off + last + 1, 0)) : it.kv;
-  const int ntot = (most + kKB - 1) / kKB;  // in the 64-key units that chunks are counted in
-  if (it.ch > 0 && it.ch * a.ct >= ntot) return;  // a causal block that ends before this chunk
-  const bool whole = !a.ct || ntot <= a.ct;
   const int t0 = a.ct ? it.ch * a.ct * 2 : 0;
-  const int t1 = min((most + kFK - 1) / kFK, a.ct ? t0 + 2 * a.ct : INT32_MAX);
 
   // ---- tiles: two 16-row halves (a page holds 16 tokens at least), each four 1-KiB pieces
   const uint32_t ldb = (uint32_t)(a.ldk * 2);
@@ -61,6 +54,28 @@ __global__ void __launch_bounds__(64 * NW) attn_seq_few_kernel(SeqArgs a) {
       pg[h] = id >= 0 && id < a.pages ? id : -1;
     }
   };
+  // table entries and q are asked for before anything looks at the sequence's length, which arrives with them
+  if constexpr (PAGED) pages(tb);
+  bf16x8_t qf[MT][NK];
+  int toks[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int r = min(row0 + 16 * mt + ql, rows - 1), head = hk * a.G + r % a.G;
+    toks[mt] = r / a.G;
+    const bf16_t* qr = a.q + (int64_t)(it.start + toks[mt]) * a.ldq + (int64_t)head * a.hsq;
+#pragma unroll
+    for (int ks = 0; ks < NK; ++ks) {
+      qf[mt][ks] = bf16x8_t{};
+      if (32 * ks + 8 * g < a.Dh) qf[mt][ks] = *(const bf16x8_t*)(qr + 32 * ks + 8 * g);
+    }
+  }
+  const int off = it.kv - it.n;
+  const int last = (min(rows, row0 + BM) - 1) / a.G;
+  const int most = a.causal ? min(it.kv, max(off + last + 1, 0)) : it.kv;
+  const int ntot = (most + kKB - 1) / kKB;  // in the 64-key units that chunks are counted in
+  if (it.ch > 0 && it.ch * a.ct >= ntot) return;  // a causal block that ends before this chunk
+  const bool whole = !a.ct || ntot <= a.ct;
+  const int t1 = min((most + kFK - 1) / kFK, a.ct ? t0 + 2 * a.ct : INT32_MAX);
   auto dma = [&](const bf16_t* base, char QIE_LDS* dst, const uint32_t (&voff)[4], int t) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -81,27 +96,12 @@ __global__ void __launch_bounds__(64 * NW) attn_seq_few_kernel(SeqArgs a) {
   };
   int t = t0 + wave;
   if (t < t1) {
-    if constexpr (PAGED) {
-      pages(t);
-      __builtin_amdgcn_s_waitcnt(0);
-    }
     dma(a.k, kt, ko, t);
     dma(a.v, vt, vo, t);
   }
-
-  bf16x8_t qf[MT][NK];
   int lim[MT];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int r = min(row0 + 16 * mt + ql, rows - 1), tok = r / a.G, head = hk * a.G + r % a.G;
-    lim[mt] = a.causal ? min(it.kv, max(off + tok + 1, 0)) : it.kv;
-    const bf16_t* qr = a.q + (int64_t)(it.start + tok) * a.ldq + (int64_t)head * a.hsq;
-#pragma unroll
-    for (int ks = 0; ks < NK; ++ks) {
-      qf[mt][ks] = bf16x8_t{};
-      if (32 * ks + 8 * g < a.Dh) qf[mt][ks] = *(const bf16x8_t*)(qr + 32 * ks + 8 * g);
-    }
-  }
+  for (int mt = 0; mt < MT; ++mt) lim[mt] = a.causal ? min(it.kv, max(off + toks[mt] + 1, 0)) : it.kv;
   const int lim0 = uni(lim[0]);
   f32x4_t o[MT][ND];
   float m_run[MT], l_run[MT];
