@@ -434,8 +434,9 @@ int qie_attention_packed_bf16(const void* q, int64_t ldq, int64_t hsq, const voi
  * ld_table apart, 0: shared), pages as in qie_rope_append_bf16. A row that sees no key is 0. Long rows are cut into chunks of keys whose
  * fp32 partials meet in `workspace` (>= qie_attention_paged_workspace bytes, 16-byte aligned, not
  * shared with a call that may run at the same time; 0 bytes, and NULL is fine, for tables of up to
- * 1024 tokens). The cuts go by the call's counts, never by the values of lengths or tables: in calls
- * of one shape a row's bits do not depend on the other sequences. */
+ * 1024 tokens). The cuts go by the call's counts, not by the values of lengths or tables: in calls of
+ * one shape a row's bits do not depend on the other sequences. Many rows over tables of more than 4096 tokens
+ * are the exception: they are cut into equal shares of the call's work, which the lengths decide. */
 int qie_attention_paged_workspace(int tokens, int seqs, int heads, int kv_heads, int head_dim, int table_width,
                                   int page_size, int64_t* bytes);
 int qie_attention_paged_bf16(const void* q, int64_t ldq, int64_t hsq, const void* k_pages, const void* v_pages,

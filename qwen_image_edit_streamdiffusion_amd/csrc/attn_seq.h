@@ -22,7 +22,8 @@ struct SeqArgs {
   int width, pages, pshift;
   // keys in chunks of ct tiles, fp32 partials (ct = 0: whole rows); rows of a block
   int ct, maxch, bm;
-  float* ws;  // O [T * H][maxch][Dh], then (m, l) [T * H][maxch][2]
+  int shares;  // 256-row blocks: work-groups that share each kv head's keys (0: a work-group a block)
+  float* ws;  // chunks: O [T * H][maxch][Dh], then (m, l) [T * H][maxch][2]; shares: attn_seq_pp.hip
 };
 
 namespace {

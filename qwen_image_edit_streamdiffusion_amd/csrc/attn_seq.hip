@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
 //     mean (1500 where causal heads share nothing and a block spans 256 tokens: 64 sequences of 1000, 24 heads over 24,
 //     687 [597 in 64-row blocks]; of 28 over 4: 551 [598]), long caches (16 x 100 new tokens over 5000: 144 [179]).
 struct SeqPlan {
-  int bm, waves, ct, maxch;
+  int bm, waves, ct, maxch, shares;
 };
 
 SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, bool causal, int64_t table_keys) {
@@ -318,7 +318,7 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, bool causal, int
   const double g16 = kv_heads * fmax(seqs, rows / 16), g32 = kv_heads * fmax(seqs, rows / 32),
                g64 = kv_heads * fmax(seqs, rows / kBM), g256 = kv_heads * fmax(1.0, rows / kPPRows);
   const int few16 = g16 <= 256 ? 8 : 4;
-  SeqPlan p{kBM, few16, 0, 1};
+  SeqPlan p{kBM, few16, 0, 1, 0};
   if (!paged) {
     if (g16 <= 512) p.bm = 16;
     else if (keys >= (causal && heads == kv_heads ? 1500 : 700) && g256 >= 200) p.bm = kPPRows;
@@ -349,6 +349,17 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, bool causal, int
   if (tiles <= 16 || (p.bm == kBM && tiles <= 32)) return p;
   const double half = per > 16 ? 0.5 * seqs * kv_heads : 0;  // sequences end inside a block
   const double groups = p.bm == 16 ? g16 + half : p.bm == 32 ? g32 + half : p.bm == kBM ? g64 / 3 : g256 + half;
+  // Many rows over more than 4096 keys, half of them kept at least: equal shares of the call's work (1500, 1100 and
+  // 700 new tokens over 24000, 11000 and 7000: 739 [836 in chunks]; 8 x 300 over 3000 and 9000: 244 [302]; of one
+  // length, 8 x 200 over 5000, 152 [136]). From 512 groups on whole blocks even out (4 x 2000 over 2000 .. 9000: 439
+  // [516 in shares]), and a single sequence's do where they fill their rounds (3500 new tokens, 383 groups, over 24000:
+  // 1047 in shares [1183]; 2340, 256 groups: 735 whole [791]).
+  const double rounds = ceil(g256 / 256);
+  if (p.bm == kPPRows && tiles > 64 && keys * seqs >= 2.0 * tokens &&
+      (seqs > 1 ? groups < 512 : g256 < 0.88 * 256 * rounds)) {
+    p.shares = kv_heads <= 256 ? 256 / kv_heads : 1;
+    return p;
+  }
   if (p.bm == kPPRows && groups >= 512) return p;
   double n = fmax(1.0, floor(256 / groups));
   if (n == 1 && 2 * groups <= 290) n = 2;
@@ -374,6 +385,7 @@ int launch_seq(SeqArgs& a, const SeqPlan& p, bool paged, hipStream_t s) {
   a.bm = p.bm;
   a.ct = p.ct;
   a.maxch = p.maxch;
+  a.shares = p.shares;
   if (p.bm != kBM) {
     const int rc = p.bm == kPPRows ? qie_launch_seq_pp(a, paged, s) : qie_launch_seq_few(a, paged, p.waves, s);
     if (rc) return rc;
@@ -384,7 +396,7 @@ int launch_seq(SeqArgs& a, const SeqPlan& p, bool paged, hipStream_t s) {
     const int rc = paged ? launch<true>(a, (unsigned)grid, s) : launch<false>(a, (unsigned)grid, s);
     if (rc) return rc;
   }
-  if (a.ct) attn_seq_join_kernel<<<(unsigned)(((int64_t)a.T * a.H + 3) / 4), 256, 0, s>>>(a);
+  if (p.ct) attn_seq_join_kernel<<<(unsigned)(((int64_t)a.T * a.H + 3) / 4), 256, 0, s>>>(a);
   return qie_last_error();
 }
 
@@ -424,7 +436,8 @@ extern "C" int qie_attention_paged_workspace(int tokens, int seqs, int heads, in
   QIE_CHECK_ARG(bytes && tokens >= 0 && seqs > 0 && heads > 0 && kv_heads > 0 && head_dim > 0 && table_width > 0 &&
                 page_size > 0 && (int64_t)table_width * page_size <= INT32_MAX / 2);
   const SeqPlan p = seq_plan(tokens, seqs, heads, kv_heads, true, (int64_t)table_width * page_size);
-  *bytes = p.ct ? (int64_t)tokens * heads * p.maxch * (head_dim + 2) * 4 : 0;
+  *bytes = p.ct ? (int64_t)tokens * heads * p.maxch * (head_dim + 2) * 4
+                : (int64_t)p.shares * 2 * kv_heads * kPPRows * (head_dim + 2) * 4;
   return QIE_OK;
 }
 

@@ -29,18 +29,192 @@ __device__ __forceinline__ void rfence(T& x) {
   asm volatile("" : "+v"(x));
 }
 
-template <bool PAGED, int KS>  // KS 16-wide steps of the head (4, 6, 8): head_dim <= 16 KS
-__global__ void __launch_bounds__(512) attn_seq_pp_kernel(SeqArgs a) {
+// ---- Shares: blocks that do not fill the chip, or not evenly, are cut where the work is, not at a fixed
+// count of keys. The blocks of one kv head lie behind each other on a line, each as long as the keys that it
+// sees; work-group s of a.shares takes the s-th equal part: the end of one block, whole blocks, the
+// beginning of another. Only the first and the last leave fp32 parts (m, l, O), two slots a work-group,
+// and a second kernel joins them. Lengths are device memory, so the line is laid out here, by every wave.
+constexpr int kShareKeys = 512;  // fewest keys of a share
+constexpr int kBlockKeys = 160;  // what beginning and ending a block costs, in keys
+
+struct Line {  // a block of the line: sequence, its place on the line, the block's ends there
+  int b, start, n, kv, nblk, blk;
+  int64_t base, c0, c1;
+};
+// where block x of a sequence begins: the sum of (cost + kept + 256 (i + 1) / G) over the blocks before it
+__device__ __forceinline__ int64_t line_at(const SeqArgs& a, int n, int kv, int x) {
+  return (int64_t)x * (max(kv - n, 0) + kBlockKeys) + (int64_t)((double)((int64_t)(kPPRows / 2) * x * (x + 1)) / a.G);
+}
+__device__ __forceinline__ int64_t uni64(int64_t v) {
+  return (int64_t)(((uint64_t)(uint32_t)uni((int)(v >> 32)) << 32) | (uint32_t)uni((int)v));
+}
+__device__ __forceinline__ int64_t line_of(const SeqArgs& a, int b, int& start, int& n, int& kv) {
+  seq_span<true>(a, b, start, n, kv);
+  return line_at(a, n, kv, (n * a.G + kPPRows - 1) / kPPRows);
+}
+__device__ __forceinline__ int64_t line_length(const SeqArgs& a) {
+  int64_t v = 0;
+  for (int b = threadIdx.x & 63; b < a.B; b += 64) {
+    int start, n, kv;
+    v += line_of(a, b, start, n, kv);
+  }
+#pragma unroll
+  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m, 64);
+  return uni64(v);
+}
+__device__ __forceinline__ void line_block(const SeqArgs& a, Line& l, int x) {
+  l.blk = x;
+  l.c0 = l.base + line_at(a, l.n, l.kv, x);
+  l.c1 = l.base + line_at(a, l.n, l.kv, x + 1);
+}
+// the block that holds position at (< the line's length)
+__device__ __forceinline__ void line_seek(const SeqArgs& a, int64_t at, Line& l) {
+  const int lane = threadIdx.x & 63;
+  l.base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    int start = 0, n = 0, kv = 0;
+    int64_t c = 0;
+    if (b0 + lane < a.B) c = line_of(a, b0 + lane, start, n, kv);
+    int64_t pre = c;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int64_t w = __shfl_up(pre, m, 64);
+      if (lane >= m) pre += w;
+    }
+    const unsigned long long hit = __ballot(l.base + pre > at);
+    if (hit) {
+      const int i = __builtin_ctzll(hit);
+      l.b = b0 + i;
+      l.start = __builtin_amdgcn_readlane(start, i);
+      l.n = __builtin_amdgcn_readlane(n, i);
+      l.kv = __builtin_amdgcn_readlane(kv, i);
+      l.base += uni64(__shfl(pre - c, i, 64));
+      break;
+    }
+    l.base += uni64(__shfl(pre, 63, 64));
+  }
+  l.nblk = (l.n * a.G + kPPRows - 1) / kPPRows;
+  int lo = 0, hi = l.nblk - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (l.base + line_at(a, l.n, l.kv, mid) <= at) lo = mid;
+    else hi = mid - 1;
+  }
+  line_block(a, l, lo);
+}
+__device__ __forceinline__ bool line_next(const SeqArgs& a, Line& l) {
+  if (l.blk + 1 < l.nblk) {
+    line_block(a, l, l.blk + 1);
+    return true;
+  }
+  l.base = l.c1;
+  for (++l.b; l.b < a.B; ++l.b) {
+    seq_span<true>(a, l.b, l.start, l.n, l.kv);
+    if (l.n == 0) continue;
+    l.nblk = (l.n * a.G + kPPRows - 1) / kPPRows;
+    line_block(a, l, 0);
+    return true;
+  }
+  return false;
+}
+// 64-key tiles of a block; the tile at which position at cuts it
+__device__ __forceinline__ int line_tiles(const SeqArgs& a, const Line& l) {
+  const int last = (min(l.n * a.G, (l.blk + 1) * kPPRows) - 1) / a.G;
+  return (min(l.kv, max(l.kv - l.n + last + 1, 0)) + kKB - 1) / kKB;
+}
+__device__ __forceinline__ int line_tile(const Line& l, int64_t at, int ntot) {
+  if (at <= l.c0) return 0;
+  return at >= l.c1 ? ntot : (int)((double)(at - l.c0) * ntot / (double)(l.c1 - l.c0));
+}
+__device__ __forceinline__ int share_count(const SeqArgs& a, int64_t total) {
+  return (int)min((int64_t)a.shares, max((int64_t)1, total / kShareKeys));
+}
+// where share i of ns begins
+__device__ __forceinline__ int64_t share_cut(int64_t total, int ns, int i) { return (int64_t)((double)total * i / ns); }
+// the fp32 part of work-group sh that begins its block (first) or goes on with it
+__device__ __forceinline__ float* share_part(const SeqArgs& a, int sh, bool first, int hk) {
+  return a.ws + ((int64_t)(2 * sh + first) * a.Hk + hk) * kPPRows * (a.Dh + 2);
+}
+
+template <typename T>
+__device__ __forceinline__ T* global(T* p) {  // memory of the device, not LDS or scratch
+  return (T*)(__attribute__((address_space(1))) T*)p;
+}
+
+template <bool SHARE, bool PAGED, int KS>  // KS 16-wide steps of the head (4, 6, 8): head_dim <= 16 KS
+__global__ void __launch_bounds__(512) attn_seq_pp_kernel(SeqArgs args) {
   constexpr int ND = KS / 2;  // 32-wide blocks of the output
   constexpr int NQ = 2 * KS, NP = 4 * ND;
   __shared__ __attribute__((aligned(16))) char smem_raw[2 * kRing * kTile];  // K ring, V ring
   char QIE_LDS* smem = (char QIE_LDS*)smem_raw;
 
-  const int hk = blockIdx.x % a.Hk;
   Item it;
-  if (!find_item<PAGED, kPPRows>(a, blockIdx.x / a.Hk, it)) return;
+  // between two blocks of a share its place waits here: in scalar registers it would push the tiles'
+  // addresses out of them
+  __shared__ struct { Line line, head; int64_t end; int head_t0; } place;
+  int t0 = 0;
+  bool tail = false;
+  if constexpr (SHARE) {
+    const SeqArgs& a = args;
+    const int sh = blockIdx.x / a.Hk;
+    const int64_t total = line_length(a);
+    const int ns = share_count(a, total);
+    if (sh >= ns) return;
+    const int64_t begin = share_cut(total, ns, sh), end = share_cut(total, ns, sh + 1);
+    if (begin >= end) return;
+    Line head, line;
+    line_seek(a, begin, head);
+    line = head;
+    t0 = line_tile(head, begin, line_tiles(a, head));
+    const int head_t0 = t0;
+    if (end < total) {
+      // the beginning of the last block goes first: its tiles and then the first block's are those that the other
+      // work-groups of the sequence read at the same time (L2)
+      Line l;
+      line_seek(a, end, l);
+      if (l.c0 > begin && line_tile(l, end, line_tiles(a, l)) > 0) {
+        line = l;
+        tail = true;
+        t0 = 0;
+      }
+    }
+    if (threadIdx.x == 0) {
+      place.line = line;
+      place.head = head;
+      place.end = end;
+      place.head_t0 = head_t0;
+    }
+    __syncthreads();
+  } else {
+    if (!find_item<PAGED, kPPRows>(args, blockIdx.x / args.Hk, it)) return;
+  }
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
   const int grp = wave >> 2, hf = lane >> 5, ql = lane & 31;
+  for (;;) {
+  // a share's next block reads the arguments anew: kept over the blocks they would fill the scalar registers
+  auto fresh = [&]() -> SeqArgs {
+    if constexpr (!SHARE) return args;
+    typedef const uint32_t __attribute__((address_space(4))) Word;
+    Word* p = (Word*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    struct { uint32_t w[sizeof(SeqArgs) / 4]; } raw;
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(SeqArgs) / 4; ++i) raw.w[i] = p[i];
+    SeqArgs r = __builtin_bit_cast(SeqArgs, raw);
+    r.q = global(r.q);
+    r.out = global(r.out);
+    r.table = global(r.table);
+    r.cu = global(r.cu);
+    r.kv_lens = global(r.kv_lens);
+    r.ws = global(r.ws);
+    return r;
+  };
+  const SeqArgs a = fresh();
+  const int hk = blockIdx.x % a.Hk;
+  if constexpr (SHARE) {
+    it.b = uni(place.line.b); it.start = uni(place.line.start); it.n = uni(place.line.n); it.kv = uni(place.line.kv);
+    it.blk = uni(place.line.blk);
+  }
   const int rows = it.n * a.G;
   const int r = it.blk * kPPRows + wave * 32 + ql;
   const int rc = min(r, rows - 1);
@@ -51,10 +225,15 @@ __global__ void __launch_bounds__(512) attn_seq_pp_kernel(SeqArgs a) {
   const int last = (min(rows, (it.blk + 1) * kPPRows) - 1) / a.G;
   const int most = a.causal ? min(it.kv, max(off + last + 1, 0)) : it.kv;
   const int ntot = (most + kKB - 1) / kKB;
-  const int t0 = a.ct ? it.ch * a.ct : 0;
-  const int ntiles = a.ct ? min(ntot, t0 + a.ct) : ntot;
-  const bool whole = !a.ct || ntot <= a.ct;
-  if (t0 > 0 && t0 >= ntot) return;  // a causal block that ends before this chunk
+  int ntiles = ntot;
+  if constexpr (SHARE) {
+    ntiles = uni(line_tile(place.line, place.end, ntot));
+  } else if (PAGED && a.ct) {
+    t0 = it.ch * a.ct;
+    if (t0 > 0 && t0 >= ntot) return;  // a causal block that ends before this chunk
+    ntiles = min(ntot, t0 + a.ct);
+  }
+  const bool whole = SHARE ? t0 == 0 && ntiles == ntot : !PAGED || !a.ct || ntot <= a.ct;
 
   bf16x8_t qf[KS];
   f32x16_t s[2], o[ND];
@@ -306,24 +485,32 @@ __global__ void __launch_bounds__(512) attn_seq_pp_kernel(SeqArgs a) {
 #pragma unroll
     for (int db = 0; db < ND; ++db) asm volatile("s_nop 15\n\ts_nop 7" : "+v"(o[db]));
   }
+  const SeqArgs e = fresh();
   const float l = l_run + __shfl_xor(l_run, 32, 64);
-  if (r >= rows) return;
-  if (!whole) {
-    const int64_t pi = ((int64_t)(it.start + tok) * a.H + head) * a.maxch + it.ch;
-    float* po = a.ws + pi * a.Dh;
-    float* pml = a.ws + (int64_t)a.T * a.H * a.maxch * a.Dh + pi * 2;
+  if (r < rows && !whole && t0 < ntiles) {
+    const int br = wave * 32 + ql;  // row of the block
+    float *po, *pml;
+    if constexpr (SHARE) {
+      float* part = share_part(e, blockIdx.x / e.Hk, t0 == 0, hk);
+      po = part + br * e.Dh;
+      pml = part + kPPRows * e.Dh + 2 * br;
+    } else {
+      const int64_t pi = ((int64_t)(it.start + tok) * e.H + head) * e.maxch + it.ch;
+      po = e.ws + pi * e.Dh;
+      pml = e.ws + (int64_t)e.T * e.H * e.maxch * e.Dh + pi * 2;
+    }
 #pragma unroll
     for (int db = 0; db < ND; ++db)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        if (32 * db + 8 * g < a.Dh)
+        if (32 * db + 8 * g < e.Dh)
           *(f32x4_t*)(po + 32 * db + 8 * g + 4 * hf) =
               f32x4_t{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
     if (hf == 0) *(f32x2_t*)pml = f32x2_t{m_run, l};
-    return;
   }
+  if (r < rows && whole) {
   const float inv = l == 0.f ? 0.f : 1.0f / l;  // no key seen: o is 0 as well
-  bf16_t* dst = a.out + (int64_t)(it.start + tok) * a.ldo + (int64_t)head * a.hso;
+  bf16_t* dst = e.out + (int64_t)(it.start + tok) * e.ldo + (int64_t)head * e.hso;
   // lane (ql, hf) holds d = 32 db + 8 g + 4 hf + 0..3; a swap of halves for two g gives 16-byte stores
 #pragma unroll
   for (int db = 0; db < ND; ++db)
@@ -335,16 +522,94 @@ __global__ void __launch_bounds__(512) attn_seq_pp_kernel(SeqArgs a) {
       const uint32_t w3 = pack2(o[db][4 * g + 6] * inv, o[db][4 * g + 7] * inv);
       const auto sx = __builtin_amdgcn_permlane32_swap(w0, w2, false, false);
       const auto sy = __builtin_amdgcn_permlane32_swap(w1, w3, false, false);
-      if (32 * db + 8 * g + 8 * hf < a.Dh)
+      if (32 * db + 8 * g + 8 * hf < e.Dh)
         *(u32x4_t*)(dst + 32 * db + 8 * g + 8 * hf) = u32x4_t{sx[0], sy[0], sx[1], sy[1]};
     }
+  }
+  if constexpr (!SHARE) return;
+  Line line = place.line;
+  int64_t end = place.end;
+  bool more = true;
+  if (tail) {
+    end = line.c0;
+    line = place.head;
+    t0 = uni(place.head_t0);
+    tail = false;
+  } else {
+    more = line.c1 < end && line_next(e, line);
+    t0 = 0;
+  }
+  __syncthreads();  // the rings are free, the place is read
+  if (!more) return;
+  if (threadIdx.x == 0) {
+    place.line = line;
+    place.end = end;
+  }
+  __syncthreads();
+  }
 }
 
-template <bool PAGED>
+// Joins a block's parts: o = sum_p w_p o_p / sum_p w_p l_p, w_p = exp2((m_p - max m) c). Work-groups
+// [kJoinSplit (s - 1), ..) of a kv head look at the cut between shares s - 1 and s and join the block that it
+// cuts first; a wave eight rows, two elements a lane.
+constexpr int kJoinRows = 8, kJoinSplit = kPPRows / (4 * kJoinRows);
+__global__ void __launch_bounds__(256) attn_seq_join_shares_kernel(SeqArgs a) {
+  const int hk = blockIdx.x % a.Hk, u = blockIdx.x / a.Hk, s = 1 + u / kJoinSplit;
+  const int64_t total = line_length(a);
+  const int ns = share_count(a, total);
+  if (s >= ns) return;
+  auto cut = [&](int i) { return share_cut(total, ns, i); };
+  Line l;
+  line_seek(a, cut(s), l);
+  const int ntot = line_tiles(a, l), t = line_tile(l, cut(s), ntot);
+  if (t == 0 || t == ntot || line_tile(l, cut(s - 1), ntot) > 0) return;
+  const int lane = threadIdx.x & 63, d = 2 * lane < a.Dh ? 2 * lane : 0;
+  const int rows = min(kPPRows, l.n * a.G - l.blk * kPPRows);
+  const int br = kJoinRows * (4 * (u % kJoinSplit) + uni(threadIdx.x >> 6));  // rows br ..
+  if (br >= rows) return;
+  float m[kJoinRows], L[kJoinRows], o0[kJoinRows], o1[kJoinRows];
+#pragma unroll
+  for (int j = 0; j < kJoinRows; ++j) {
+    m[j] = kLow;
+    L[j] = o0[j] = o1[j] = 0.f;
+  }
+  for (int i0 = s - 1; i0 < ns && cut(i0) < l.c1; i0 += 64) {
+    const int me = i0 + lane;  // a lane looks whether its share left a part
+    const bool has = me < ns && cut(me) < l.c1 && (me < s || line_tile(l, cut(me), ntot) < line_tile(l, cut(me + 1), ntot));
+    for (unsigned long long left = __ballot(has); left; left &= left - 1) {
+      const int i = i0 + __builtin_ctzll(left);
+      const float* p = share_part(a, i, i < s, hk);
+      f32x2_t ml[kJoinRows], v[kJoinRows];
+#pragma unroll
+      for (int j = 0; j < kJoinRows; ++j) {  // rows past the block's last: their part is there, and unread below
+        ml[j] = *(const f32x2_t*)(p + kPPRows * a.Dh + 2 * (br + j));
+        v[j] = *(const f32x2_t*)(p + (br + j) * a.Dh + d);
+      }
+#pragma unroll
+      for (int j = 0; j < kJoinRows; ++j) {
+        const float mn = fmaxf(m[j], ml[j][0]);
+        const float f = __builtin_amdgcn_exp2f((m[j] - mn) * a.c), w = __builtin_amdgcn_exp2f((ml[j][0] - mn) * a.c);
+        m[j] = mn;
+        L[j] = __builtin_fmaf(w, ml[j][1], L[j] * f);
+        o0[j] = __builtin_fmaf(w, v[j][0], o0[j] * f);
+        o1[j] = __builtin_fmaf(w, v[j][1], o1[j] * f);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kJoinRows; ++j) {
+    const float inv = L[j] == 0.f ? 0.f : 1.0f / L[j];
+    const int r = l.blk * kPPRows + br + j, tok = r / a.G, head = hk * a.G + r % a.G;
+    if (br + j < rows && 2 * lane < a.Dh)
+      *(uint32_t*)(a.out + (int64_t)(l.start + tok) * a.ldo + (int64_t)head * a.hso + d) = pack2(o0[j] * inv, o1[j] * inv);
+  }
+}
+
+template <bool SHARE, bool PAGED>
 int launch(const SeqArgs& a, unsigned grid, hipStream_t s) {
-  if (a.Dh <= 64) attn_seq_pp_kernel<PAGED, 4><<<grid, 512, 0, s>>>(a);
-  else if (a.Dh <= 96) attn_seq_pp_kernel<PAGED, 6><<<grid, 512, 0, s>>>(a);
-  else attn_seq_pp_kernel<PAGED, 8><<<grid, 512, 0, s>>>(a);
+  if (a.Dh <= 64) attn_seq_pp_kernel<SHARE, PAGED, 4><<<grid, 512, 0, s>>>(a);
+  else if (a.Dh <= 96) attn_seq_pp_kernel<SHARE, PAGED, 6><<<grid, 512, 0, s>>>(a);
+  else attn_seq_pp_kernel<SHARE, PAGED, 8><<<grid, 512, 0, s>>>(a);
   return qie_last_error();
 }
 
@@ -352,7 +617,11 @@ int launch(const SeqArgs& a, unsigned grid, hipStream_t s) {
 
 int qie_launch_seq_pp(const SeqArgs& a, bool paged, hipStream_t s) {
   const int64_t rb = (int64_t)a.T * a.G / kPPRows + a.B;  // at least the row blocks of any lengths
-  const int64_t grid = rb * (a.ct ? a.maxch : 1) * a.Hk;
-  if (grid > INT32_MAX) return QIE_ERR_UNSUPPORTED;
-  return paged ? launch<true>(a, (unsigned)grid, s) : launch<false>(a, (unsigned)grid, s);
+  const int64_t grid = rb * a.maxch * a.Hk;
+  if (grid > INT32_MAX || (int64_t)a.shares * a.Hk * kJoinSplit > INT32_MAX) return QIE_ERR_UNSUPPORTED;
+  if (!a.shares) return paged ? launch<false, true>(a, (unsigned)grid, s) : launch<false, false>(a, (unsigned)grid, s);
+  const int rc = launch<true, true>(a, (unsigned)(a.shares * a.Hk), s);
+  if (rc || a.shares == 1) return rc;
+  attn_seq_join_shares_kernel<<<(unsigned)((a.shares - 1) * a.Hk * kJoinSplit), 256, 0, s>>>(a);
+  return qie_last_error();
 }

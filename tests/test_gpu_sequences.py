@@ -334,7 +334,12 @@ PAGED = [([1], [1], 1, 1, 64, 16, "heads"), ([1, 1, 1], [5, 700, 64], 28, 4, 128
          ([2] * 67, [40] * 66 + [3000], 20, 1, 128, 64, "heads"), ([600, 900], [5000, 2500], 28, 4, 128, 64, "heads"),
          ([300, 200], [300, 400], 28, 4, 128, 16, "rows"), ([300, 200], [300, 400], 28, 4, 64, 64, "heads"),
          ([8] * 20, [8] * 19 + [3000], 28, 4, 128, 16, "heads"), ([700, 900], [700, 3000], 16, 2, 80, 32, "rows"),
-         ([30], [400], 40, 1, 128, 64, "heads"), ([2500], [2500], 16, 2, 64, 16, "heads")]
+         ([30], [400], 40, 1, 128, 64, "heads"), ([2500], [2500], 16, 2, 64, 16, "heads"),
+         # 256-row blocks in equal shares of the work: uneven lengths, none, fewer kept than new, one block cut often
+         ([400, 5, 0, 360], [4500, 900, 40, 380], 16, 2, 128, 64, "heads"), ([400, 380], [4500, 4200], 14, 2, 72, 16, "rows"),
+         ([900, 300, 1], [5000, 0, 4000], 16, 2, 64, 32, "heads"), ([1000, 40], [1000, 4300], 16, 2, 128, 64, "heads"),
+         ([800], [4800], 20, 1, 128, 16, "rows"), ([10] * 70, [70] * 69 + [4200], 64, 1, 64, 16, "heads"),
+         ([900, 700], [20, 5000], 24, 3, 96, 128, "heads")]
 
 
 @pytest.mark.parametrize("new,kv,H,Hk,Dh,P,layout", PAGED)
@@ -366,7 +371,7 @@ def test_attention_paged_rows_do_not_depend_on_other_sequences(new, kv):
     assert torch.equal(other[mid], got[mid]) and not torch.equal(other[:new[0]], got[:new[0]])
 
 
-@pytest.mark.parametrize("new,kv,H,Hk", [(60, 100, 28, 4), (7, 2000, 6, 1), (9, 2600, 28, 4), (400, 450, 28, 4), (30, 3000, 40, 1),
+@pytest.mark.parametrize("new,kv,H,Hk", [(700, 5000, 28, 4), (60, 100, 28, 4), (7, 2000, 6, 1), (9, 2600, 28, 4), (400, 450, 28, 4), (30, 3000, 40, 1),
                                          (1200, 3000, 28, 4)])
 def test_attention_paged_nonfinite_later_keys(new, kv, H, Hk):
     """Infinities and NaN of a later key of the same chunk do not reach the queries before it."""
@@ -563,7 +568,8 @@ def test_other_stream():
     assert torch.equal(got, ref)
 
 
-@pytest.mark.parametrize("new,kv", [([1, 1, 1], [3000, 5, 700]), ([40, 3, 60], [3000, 300, 60]), ([700, 5, 900], [3000, 300, 900])])
+@pytest.mark.parametrize("new,kv", [([1, 1, 1], [3000, 5, 700]), ([40, 3, 60], [3000, 300, 60]), ([700, 5, 900], [3000, 300, 900]),
+                                    ([700, 5, 900], [5000, 300, 900])])
 def test_two_streams_and_in_place(new, kv):
     """Two calls at once, each with its own workspace, and a call whose out is q: bitwise the call alone."""
     ops = _ops()
