@@ -236,7 +236,9 @@ __global__ void __launch_bounds__(256, NK == 4 ? 3 : 4) attn_seq_kernel(SeqArgs 
 }
 
 // Joins the chunks of a row: o = sum_c w_c o_c / sum_c w_c l_c, w_c = exp2((m_c - max m) c). One wave a
-// (token, head); the rows that one chunk held are written already.
+// (token, head); the rows that one chunk held are written already. Bound by the latency of its loads, one behind
+// the other: the length, then a lane's (m, l) and the first eight chunks' parts together, then eight at a time
+// ahead of their use.
 __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + uni(threadIdx.x >> 6);
@@ -244,16 +246,20 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
   const int token = (int)(row / a.H), head = (int)(row - (int64_t)token * a.H);
   // the sequence of this token: the last one that starts at or before it
   int b = -1, start = 0, n = 0, kv = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
+  if (!a.cu) {
+    b = token;
+    seq_span<true>(a, b, start, n, kv);
+  }
+  for (int b0 = 0; a.cu && b0 < a.B; b0 += 64) {
     int s0 = 0, n0 = 0, k0 = 0;
     if (b0 + lane < a.B) seq_span<true>(a, b0 + lane, s0, n0, k0);
     const unsigned long long hit = __ballot(b0 + lane < a.B && s0 <= token && token < s0 + n0);
     if (hit) {
       const int l = __builtin_ctzll(hit);
       b = b0 + l;
-      start = uni(__shfl(s0, l, 64));
-      n = uni(__shfl(n0, l, 64));
-      kv = uni(__shfl(k0, l, 64));
+      start = __builtin_amdgcn_readlane(s0, l);
+      n = __builtin_amdgcn_readlane(n0, l);
+      kv = __builtin_amdgcn_readlane(k0, l);
       break;
     }
   }
@@ -262,30 +268,42 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
   const int r = (token - start) * a.G + head % a.G, blk = r / a.bm;
   const int last = (min(n * a.G, (blk + 1) * a.bm) - 1) / a.G;
   const int most = a.causal ? min(kv, max(kv - n + last + 1, 0)) : kv;
-  const int ntot = (most + kKB - 1) / kKB, nch = (ntot + a.ct - 1) / a.ct;
+  const int ntot = (most + kKB - 1) / kKB, nch = uni((ntot + a.ct - 1) / a.ct);
   if (nch <= 1) return;
   const float* pml = a.ws + (int64_t)a.T * a.H * a.maxch * a.Dh + row * a.maxch * 2;
-  const float* po = a.ws + row * a.maxch * a.Dh;
-  float mx = kLow;
-  for (int c = lane; c < nch; c += 64) mx = fmaxf(mx, pml[2 * c]);
+  const int d = 2 * lane;
+  const float* po = a.ws + row * a.maxch * a.Dh + (d < a.Dh ? d : 0);
+  constexpr int kAhead = 8;
+  f32x2_t ml = f32x2_t{kLow, 0.f}, v[kAhead], w[kAhead];
+  if (lane < nch) ml = *(const f32x2_t*)(pml + 2 * lane);
+  auto fetch = [&](f32x2_t* to, int from) {  // past the last chunk: the last once more, its weight is 0 then
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) to[i] = *(const f32x2_t*)(po + (int64_t)min(from + i, nch - 1) * a.Dh);
+  };
+  fetch(v, 0);
+  float mx = ml[0];
+  for (int c = lane + 64; c < nch; c += 64) mx = fmaxf(mx, pml[2 * c]);
   mx = wave_max(mx);
   float l = 0.f, o0 = 0.f, o1 = 0.f;
-  const int d = 2 * lane;
   for (int c0 = 0; c0 < nch; c0 += 64) {  // a lane weighs a chunk, then all lanes add 64 chunks' rows
-    float w = 0.f;
-    if (c0 + lane < nch) {
-      const f32x2_t q = *(const f32x2_t*)(pml + 2 * (c0 + lane));
-      w = __builtin_amdgcn_exp2f((q[0] - mx) * a.c);
-      l = __builtin_fmaf(w, q[1], l);
+    if (c0 > 0) {
+      ml = f32x2_t{kLow, 0.f};
+      if (c0 + lane < nch) ml = *(const f32x2_t*)(pml + 2 * (c0 + lane));
     }
+    const float wt = c0 + lane < nch ? __builtin_amdgcn_exp2f((ml[0] - mx) * a.c) : 0.f;
+    l = __builtin_fmaf(wt, ml[1], l);
     const int n64 = min(64, nch - c0);
-    const float* pc = po + (int64_t)c0 * a.Dh + (d < a.Dh ? d : 0);
-#pragma unroll 8
-    for (int c = 0; c < n64; ++c) {
-      const float wc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), c));
-      const f32x2_t v = *(const f32x2_t*)(pc + (int64_t)c * a.Dh);
-      o0 = __builtin_fmaf(wc, v[0], o0);
-      o1 = __builtin_fmaf(wc, v[1], o1);
+    for (int c = 0; c < n64; c += kAhead) {
+      fetch(w, c0 + c + kAhead);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const float wc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wt), c + i));
+        if (c + i < n64) {
+          o0 = __builtin_fmaf(wc, v[i][0], o0);
+          o1 = __builtin_fmaf(wc, v[i][1], o1);
+        }
+        v[i] = w[i];
+      }
     }
   }
   l = wave_sum(l);
