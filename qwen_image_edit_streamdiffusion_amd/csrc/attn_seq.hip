@@ -356,13 +356,14 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, bool causal, int
     p.bm = keys <= 2048 && g256 < 200 ? kBM : kPPRows;
   }
   // Cuts: groups that do not fill the chip share a row's keys, in chunks whose fp32 parts a second kernel
-  // joins: as many as fit 256 CUs at once (1000 new tokens over 5000 keys, two of 40 tiles: 99 [uncut 138, three
-  // chunks 124]; three 64-row work-groups fit a CU), of 8 tiles at least. Up to 1024 keys, none (one
-  // token: 10.1 in one launch [10.9 in two]). Few rows: 1.4 sqrt(tiles) tiles at least, where a chunk's time
-  // and the join's meet (one token over 32768 keys: 26.4 with 16 or 32 tiles [34 with 8 or 64]). Long tables are
-  // cut all the same, so that a long sequence among short ones is shared (48 tokens over 900 .. 32768 keys:
-  // 298 [840 uncut]): into 32 tiles (4 and 16 new tokens over 20000 keys of 16 sequences: 104 and 167 [132 and 240
-  // with 64]), 64 where there is one sequence or the groups fill the chip without a cut.
+  // joins: as many as fit 256 CUs at once (1000 new tokens over 5000 keys, two of 40 tiles: 98 [uncut 138, three
+  // chunks 124]; three 64-row work-groups fit a CU), of 8 tiles at least. Up to 1024 keys, none (one token over
+  // 1000: 9.8 in one launch [10.4 in two]). Few rows: 0.6 sqrt(tiles) tiles and 4 at least, where a chunk's time
+  // and the join's meet (one token over 2000, 8000 and 32768 keys: 9.9, 11.6 and 19.5 [11.4, 13.8 and 21.7 with 8 and
+  // 1.4 sqrt(tiles)]). Long tables are cut all the same, so that a long sequence among short ones is shared (48
+  // tokens over 900 .. 32768 keys: 291 [840 uncut]): into 32 tiles (4 and 16 new tokens over 20000 keys of 16
+  // sequences: 104 and 167 [132 and 240 with 64]), 64 where there is one sequence or the groups fill the chip
+  // without a cut.
   const double tiles = (double)((table_keys + kKB - 1) / kKB);
   if (tiles <= 16 || (p.bm == kBM && tiles <= 32)) return p;
   const double half = per > 16 ? 0.5 * seqs * kv_heads : 0;  // sequences end inside a block
@@ -381,7 +382,7 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, bool causal, int
   if (p.bm == kPPRows && groups >= 512) return p;
   double n = fmax(1.0, floor(256 / groups));
   if (n == 1 && 2 * groups <= 290) n = 2;
-  const double low = p.bm < kBM ? fmax(8.0, 1.4 * sqrt(tiles)) : 8;
+  const double low = p.bm < kBM ? fmax(4.0, 0.6 * sqrt(tiles)) : 8;
   double ct = fmax(tiles / n, low);
   if (per <= 64 || tiles > 128) ct = fmin(ct, groups >= 256 || (per > 64 && seqs == 1) ? 64 : fmax(32.0, low));
   if (tiles > ct) {
