@@ -1,6 +1,6 @@
 // Shared pieces of the attention over sequences (attn_seq.hip: 64-row blocks, joins and dispatch;
-// attn_seq_pp.hip: 256-row blocks): arguments, where a work-group's item lies, tile loads, and what
-// keeps infinities and NaN of masked keys away from the rows that do not see them.
+// attn_seq_few.hip: 16 and 32; attn_seq_pp.hip: 256): arguments, where a work-group's item lies, tile loads,
+// and what keeps infinities and NaN of masked keys away from the rows that do not see them.
 #pragma once
 #include "qie_common.h"
 
@@ -28,7 +28,7 @@ struct SeqArgs {
 
 namespace {
 
-constexpr int kKB = 64;      // keys of a tile
+constexpr int kKB = 64;      // keys of a tile, here the unit in which chunks are counted
 constexpr int kRowB = 256;   // LDS row: 128 elements, narrower heads leave zeros
 constexpr int kTile = kKB * kRowB;
 constexpr float kLow = -1e30f;     // "no key yet": finite, so that exp2(-inf - kLow) is 0 and not NaN

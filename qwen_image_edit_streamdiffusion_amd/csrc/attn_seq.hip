@@ -9,13 +9,18 @@
 // matrix instruction, and a causal diagonal is G times narrower in rows.
 //
 // attn_seq_kernel: one work-group = 4 waves = 64 rows of one (sequence, kv head), 32-key tiles,
-// double-buffered in LDS by buffer_load ... lds (32 KiB, four work-groups a CU: short sequences are
+// double-buffered in LDS by buffer_load ... lds (32 KiB, three or four work-groups a CU: short sequences are
 // bound by the latency of a chain of loads, which other work-groups fill). Per wave and tile, 16 rows:
 //   S^T = K Q^T (mfma 16x16x32, K rows by ds_read_b128 from an XOR-swizzled image, Q^T in registers)
 //   a lane holds 8 keys of one row: online softmax in log2 units (running max and sum in fp32, the
-//   rescale only when a max grows by more than 2^8), P rounded to bf16 for the second product
+//   rescale only when a max grows by more than 2^8), P rounded to bf16 for the second product, as the
+//   matrix instruction takes it (2^-9 of the largest |v| a row's result)
 //   O^T += V^T P^T (V^T by ds_read_b64_tr_b16; the S^T registers are the P^T operand)
-// Rows past a tile's last key come from the buffer's range check as zeros.
+// Rows past a tile's last key come from the buffer's range check as zeros. Measured: 64 windows of 16 .. 64
+// rows, 16 heads of 80, 10.2 us (2.5 TB/s); six causal prompts of 70 .. 420, 28 heads over 4, 16.5 us, whose
+// longest block walks 14 tiles of 0.8 us one behind the other; 16 prompts of 400 42 us. Tried and slower or
+// equal: 64-key tiles, three stages with one barrier a tile, 32 rows a wave, two groups of waves a block that
+// share its keys.
 #include <cmath>
 
 #include "attn_seq.h"
@@ -317,8 +322,10 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
 // unless said, the other side in brackets.
 //   few rows (attn_seq_few), 16-row blocks: up to 256 groups with eight waves each (one prompt of 100
 //     tokens 6.6 [9.2 in 64-row blocks]), up to 512 with four, two a CU (one prompt of 200: 8.4 [11.6 with
-//     eight]). 32-row blocks where 16-row ones would be more, or read a long cache again and again (4 new
-//     tokens over 20000 keys of 16 sequences: 104 [150]).
+//     eight]), and more than that over up to 1500 keys (80 tokens of 24 heads over 24, caches of 20, 300 and 1000:
+//     19, 53 and 176 [32, 69 and 180 with eight; over 8000 1287 with four, 1277 with eight]). 32-row blocks where
+//     16-row ones would be more, or read a long cache again and again (4 new tokens over 20000 keys of 16
+//     sequences: 104 [150]).
 //   64-row blocks (attn_seq): shorter packed sequences (16 prompts of 400: 42 [52 in 256-row blocks]), a short
 //     cache's many rows (16 x 100 new tokens over 300: 20 [25]), and 33 .. 64 rows of a sequence over a long one (16 x
 //     8 new tokens over 20000: 107 [156 in 32-row blocks]).
@@ -344,7 +351,7 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, bool causal, int
   }
   if (per <= 16) {
     p.bm = 16;
-    p.waves = 8;
+    p.waves = keys <= 1536 ? few16 : 8;
   } else if (keys <= 512) {
     p.bm = g16 <= 512 ? 16 : kBM;
   } else if (per > 32 && per <= 64 && g32 * keys > 3e5) {
