@@ -122,12 +122,18 @@ __device__ __forceinline__ bool find_item(const SeqArgs& a, int idx, Item& it) {
   return false;
 }
 
-// max / sum over the four lanes that hold a row (lanes l, l ^ 16, l ^ 32, l ^ 48) without LDS
+// max / sum over the four lanes that hold a row (lanes l, l ^ 16, l ^ 32, l ^ 48) without LDS. The
+// instruction itself: fmaxf first quiets the operands that came as integers, two more instructions a step
+__device__ __forceinline__ float max_of(uint32_t x, uint32_t y) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(y));
+  return r;
+}
 __device__ __forceinline__ float quad_max(float v) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  v = max_of(a[0], a[1]);
   const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+  return max_of(b[0], b[1]);
 }
 __device__ __forceinline__ float quad_sum(float v) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);

@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(512) attn_seq_pp_kernel(SeqArgs args) {
       mma32(o[(i - NQ) % ND], A, pf[(i - NQ) / ND]);
     }
   };
-  constexpr int PF = 5;  // operand prefetch distance in products
+  constexpr int PF = 6;  // operand prefetch distance in products
   bf16x8_t A[8];
   // products [i0, i1) with the operands up to i2 (the next part's first ones) read on the way
   auto products = [&](auto i0_t, auto i1_t, auto i2_t, int tk, int tv) {
