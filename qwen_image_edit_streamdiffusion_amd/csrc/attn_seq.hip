@@ -140,6 +140,21 @@ __global__ void __launch_bounds__(256, NK == 4 ? 3 : 4) attn_seq_kernel(SeqArgs 
         s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, qf[ks], s[kb], 0, 0, 0);
       }
     }
+    // V^T fragment: lane's d = 16 db + ql, keys 4 g + 0..3 and 16 further
+    auto vfrag = [&](int db) -> bf16x8_t {
+      const int row = 4 * g + (ql >> 2);
+      const int ch = (2 * db + ((ql & 3) >> 1)) ^ ((row & 7) << 1);
+      const char QIE_LDS* p0 = vt + row * kRowB + (ch << 4) + 8 * (ql & 1);
+      const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t QIE_LDS*)p0);
+      const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t QIE_LDS*)(p0 + 16 * kRowB));
+      return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    bf16x8_t vv[ND];
+    if constexpr (!MASKED) {
+#pragma unroll
+      for (int db = 0; db < ND; ++db) vv[db] = vfrag(db);
+      asm volatile("" ::: "memory");
+    }
     const int kv0 = t * KT;
     if constexpr (MASKED) {
 #pragma unroll
@@ -172,15 +187,6 @@ __global__ void __launch_bounds__(256, NK == 4 ? 3 : 4) attn_seq_kernel(SeqArgs 
     }
     l_run += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
     asm volatile("" : "+v"(l_run));  // here, not behind the products
-    // V^T fragment: lane's d = 16 db + ql, keys 4 g + 0..3 and 16 further
-    auto vfrag = [&](int db) -> bf16x8_t {
-      const int row = 4 * g + (ql >> 2);
-      const int ch = (2 * db + ((ql & 3) >> 1)) ^ ((row & 7) << 1);
-      const char QIE_LDS* p0 = vt + row * kRowB + (ch << 4) + 8 * (ql & 1);
-      const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t QIE_LDS*)p0);
-      const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t QIE_LDS*)(p0 + 16 * kRowB));
-      return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-    };
     // 0 * inf and 0 * NaN: a masked key's V must not reach the rows that do not see it
     bool bad = false;
     if constexpr (MASKED) {
@@ -210,7 +216,7 @@ __global__ void __launch_bounds__(256, NK == 4 ? 3 : 4) attn_seq_kernel(SeqArgs 
       }
     } else {
 #pragma unroll
-      for (int db = 0; db < ND; ++db) o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vfrag(db), pf, o[db], 0, 0, 0);
+      for (int db = 0; db < ND; ++db) o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(MASKED ? vfrag(db) : vv[db], pf, o[db], 0, 0, 0);
     }
     if (t + 1 == t1) return;
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // this tile's stage is free
