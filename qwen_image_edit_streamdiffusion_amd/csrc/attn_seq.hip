@@ -30,8 +30,8 @@ namespace {
 
 constexpr int kBM = 64;  // rows of a work-group
 
-template <bool PAGED, int NK>  // NK 32-wide steps of the head: head_dim <= 32 NK
-__global__ void __launch_bounds__(256, NK == 4 ? 3 : 4) attn_seq_kernel(SeqArgs a) {
+template <bool PAGED, int NK, int WGS>  // NK 32-wide steps of the head: head_dim <= 32 NK; work-groups of a CU
+__global__ void __launch_bounds__(256, WGS) attn_seq_kernel(SeqArgs a) {
   constexpr int ND = 2 * NK;     // 16-wide blocks of the output
   constexpr int KT = 32, KB = KT / 16, NP = KT / 16;  // keys of a tile, their blocks, pieces of a wave
   constexpr int TILE = KT * kRowB;
@@ -418,9 +418,12 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, bool causal, int
 
 template <bool PAGED>
 int launch(const SeqArgs& a, unsigned grid, hipStream_t s) {
-  if (a.Dh <= 64) attn_seq_kernel<PAGED, 2><<<grid, 256, 0, s>>>(a);
-  else if (a.Dh <= 96) attn_seq_kernel<PAGED, 3><<<grid, 256, 0, s>>>(a);
-  else attn_seq_kernel<PAGED, 4><<<grid, 256, 0, s>>>(a);
+  // 128-wide heads fit four work-groups a CU with a register spilled (where V holds infinities): taken where more
+  // than three a CU are there (64 prompts of 400: 196 us [211 with three]; six prompts 16.7 [16.5])
+  if (a.Dh <= 64) attn_seq_kernel<PAGED, 2, 4><<<grid, 256, 0, s>>>(a);
+  else if (a.Dh <= 96) attn_seq_kernel<PAGED, 3, 4><<<grid, 256, 0, s>>>(a);
+  else if (grid > 3 * 256) attn_seq_kernel<PAGED, 4, 4><<<grid, 256, 0, s>>>(a);
+  else attn_seq_kernel<PAGED, 4, 3><<<grid, 256, 0, s>>>(a);
   return qie_last_error();
 }
 
