@@ -346,24 +346,34 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
 //   64-row blocks (attn_seq): shorter packed sequences (16 prompts of 400: 42 [52 in 256-row blocks]), a short
 //     cache's many rows (16 x 100 new tokens over 300: 20 [25]), and 33 .. 64 rows of a sequence over a long one (16 x
 //     8 new tokens over 20000: 107 [156 in 32-row blocks]).
-//   256-row blocks (attn_seq_pp) where there are about 200 of them: packed sequences of 700 tokens in the
-//     mean (1500 where causal heads share nothing and a block spans 256 tokens: 64 sequences of 1000, 24 heads over 24,
-//     687 [597 in 64-row blocks]; of 28 over 4: 551 [598]), long caches (16 x 100 new tokens over 5000: 144 [179]).
+//   256-row blocks (attn_seq_pp) for packed sequences where there are 200 of them, their rounds are full enough, and the
+//     mean length is 700 (10 x 1000: 122 [126 in 64-row blocks]; 5 x 2000: 173 [191]; 1500 where causal heads share
+//     nothing and a block spans 256 tokens: 10 x 1000, 24 heads over 24, 118 [104]). Narrow heads cost them as much as
+//     wide ones: from 1800 causal or 1000 full rows at 65 .. 96 (7 x 1500, 16 heads of 80: 100 [85]; 4 x 3000: 145 [153];
+//     full 7 x 1500: 122 [135]), from 5000 or 3500 at 64 (8 heads, 4 x 3000: 90 [75], 4 x 8000: 374 [402]; full 4 x 4000:
+//     164 [197]; shared heads from 3500 or 1500: 12 over 4, 4 x 4000 151 [156]). Over a cache, for more than 2048 keys (6 x 600 over 3000: 180 [188]; 3 x 1500 over 1500: 85 [76]; heads
+//     of 64 4096), where little of a block is padding: a sixth (6 x 600 over 3000, 16 heads of 80, 18 blocks for 14:
+//     160 [106]), a third where shares even out the rest (10 of up to 758 over up to 9770: 402 [458]).
 struct SeqPlan {
   int bm, waves, ct, maxch, shares;
 };
 
-SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, bool causal, int64_t table_keys) {
+SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, int head_dim, bool causal, int64_t table_keys) {
   const bool paged = table_keys > 0;
   const double rows = (double)tokens * (heads / kv_heads), per = rows / seqs;  // in all, of a sequence
   const double keys = paged ? (double)table_keys : (double)tokens / seqs;
   const double g16 = kv_heads * fmax(seqs, rows / 16), g32 = kv_heads * fmax(seqs, rows / 32),
                g64 = kv_heads * fmax(seqs, rows / kBM), g256 = kv_heads * fmax(1.0, rows / kPPRows);
   const int few16 = g16 <= 256 ? 8 : 4;
+  // from what length on 256-row blocks pay, and how full their rounds of 256 are
+  const double longest = head_dim > 96  ? (causal && heads == kv_heads ? 1500 : 700)
+                         : head_dim > 64 ? (causal ? 1800 : 1000)
+                         : heads == kv_heads ? (causal ? 5000 : 3500) : (causal ? 3500 : 1500);
+  const double rounds = ceil(g256 / 256), pad = ceil(per / kPPRows) * kPPRows / per;
   SeqPlan p{kBM, few16, 0, 1, 0};
   if (!paged) {
     if (g16 <= 512) p.bm = 16;
-    else if (keys >= (causal && heads == kv_heads ? 1500 : 700) && g256 >= 200) p.bm = kPPRows;
+    else if (keys >= longest && g256 >= 200 && (g256 >= 512 || g256 >= 0.65 * 256 * rounds)) p.bm = kPPRows;
     return p;
   }
   if (per <= 16) {
@@ -377,7 +387,7 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, bool causal, int
     p.bm = g16 <= 512 && g16 * keys <= 4e5 ? 16 : 32;
     if (p.bm == 32) p.waves = 8;
   } else {
-    p.bm = keys <= 2048 && g256 < 200 ? kBM : kPPRows;
+    p.bm = keys > (head_dim > 64 ? 2048 : 4096) && pad <= (keys > 4096 ? 1.5 : 1.2) ? kPPRows : kBM;
   }
   // Cuts: groups that do not fill the chip share a row's keys, in chunks whose fp32 parts a second kernel
   // joins: as many as fit 256 CUs at once (1000 new tokens over 5000 keys, two of 40 tiles: 98 [uncut 138, three
@@ -397,7 +407,6 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, bool causal, int
   // length, 8 x 200 over 5000, 152 [136]). From 512 groups on whole blocks even out (4 x 2000 over 2000 .. 9000: 439
   // [516 in shares]), and a single sequence's do where they fill their rounds (3500 new tokens, 383 groups, over 24000:
   // 1047 in shares [1183]; 2340, 256 groups: 735 whole [791]).
-  const double rounds = ceil(g256 / 256);
   if (p.bm == kPPRows && tiles > 64 && keys * seqs >= 2.0 * tokens &&
       (seqs > 1 ? groups < 512 : g256 < 0.88 * 256 * rounds)) {
     p.shares = kv_heads <= 256 ? 256 / kv_heads : 1;
@@ -474,14 +483,14 @@ extern "C" int qie_attention_packed_bf16(const void* q, int64_t ldq, int64_t hsq
   a.B = seqs; a.T = tokens; a.H = heads; a.Hk = kv_heads; a.G = heads / kv_heads; a.Dh = head_dim;
   a.causal = causal != 0;
   a.c = scale * 1.4426950408889634f;
-  return launch_seq(a, seq_plan(tokens, seqs, heads, kv_heads, causal != 0, 0), false, (hipStream_t)stream);
+  return launch_seq(a, seq_plan(tokens, seqs, heads, kv_heads, head_dim, causal != 0, 0), false, (hipStream_t)stream);
 }
 
 extern "C" int qie_attention_paged_workspace(int tokens, int seqs, int heads, int kv_heads, int head_dim,
                                              int table_width, int page_size, int64_t* bytes) {
   QIE_CHECK_ARG(bytes && tokens >= 0 && seqs > 0 && heads > 0 && kv_heads > 0 && head_dim > 0 && table_width > 0 &&
                 page_size > 0 && (int64_t)table_width * page_size <= INT32_MAX / 2);
-  const SeqPlan p = seq_plan(tokens, seqs, heads, kv_heads, true, (int64_t)table_width * page_size);
+  const SeqPlan p = seq_plan(tokens, seqs, heads, kv_heads, head_dim, true, (int64_t)table_width * page_size);
   *bytes = p.ct ? (int64_t)tokens * heads * p.maxch * (head_dim + 2) * 4
                 : (int64_t)p.shares * 2 * kv_heads * kPPRows * (head_dim + 2) * 4;
   return QIE_OK;
@@ -517,6 +526,6 @@ extern "C" int qie_attention_paged_bf16(const void* q, int64_t ldq, int64_t hsq,
   a.kv_lens = kv_lens;
   a.width = table_width; a.pages = num_pages; a.pshift = __builtin_ctz(page_size);
   a.ws = (float*)workspace;
-  return launch_seq(a, seq_plan(tokens, seqs, heads, kv_heads, true, (int64_t)table_width * page_size), true,
+  return launch_seq(a, seq_plan(tokens, seqs, heads, kv_heads, head_dim, true, (int64_t)table_width * page_size), true,
                     (hipStream_t)stream);
 }
