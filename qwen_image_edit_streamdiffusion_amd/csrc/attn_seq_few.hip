@@ -21,7 +21,7 @@ __global__ void __launch_bounds__(64 * NW) attn_seq_few_kernel(SeqArgs a) {
   constexpr int ND = 2 * NK;
   constexpr int BM = 16 * MT;
   __shared__ __attribute__((aligned(16))) char smem_raw[NW * 2 * kFTile];
-  __shared__ float ml[NW][BM][2];
+  __shared__ __attribute__((aligned(8))) float ml[NW][BM][2];
   char QIE_LDS* smem = (char QIE_LDS*)smem_raw;
 
   const int hk = blockIdx.x % a.Hk;
@@ -237,21 +237,24 @@ __global__ void __launch_bounds__(64 * NW) attn_seq_few_kernel(SeqArgs a) {
   for (int u = threadIdx.x; u < BM * nc; u += 64 * NW) {
     const int row = u / nc, ch = u - row * nc, r = row0 + row;
     if (r >= rows) break;
+    f32x2_t mw[NW];
+    f32x4_t v[NW];
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      mw[w] = *(const f32x2_t QIE_LDS*)&ml[w][row][0];
+      v[w] = *(const f32x4_t QIE_LDS*)(smem + w * 2 * kFTile + row * 512 + ((ch ^ (row & 15)) << 4));
+    }
     float M = kLow;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[w][row][0]);
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, mw[w][0]);
     float L = 0.f;
     f32x4_t O = f32x4_t{};
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const float lw = ml[w][row][1];
-      const float f = __builtin_amdgcn_exp2f((ml[w][row][0] - M) * a.c);
-      if (lw != 0.f) {  // a wave that saw no key left nothing
-        const f32x4_t v = *(const f32x4_t QIE_LDS*)(smem + w * 2 * kFTile + row * 512 + ((ch ^ (row & 15)) << 4));
-        L = __builtin_fmaf(f, lw, L);
+      const float f = __builtin_amdgcn_exp2f((mw[w][0] - M) * a.c);  // a wave that saw no key left zeros
+      L = __builtin_fmaf(f, mw[w][1], L);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) O[i] = __builtin_fmaf(f, v[i], O[i]);
-      }
+      for (int i = 0; i < 4; ++i) O[i] = __builtin_fmaf(f, v[w][i], O[i]);
     }
     const int tok = r / a.G, head = hk * a.G + r % a.G;
     if (whole) {
