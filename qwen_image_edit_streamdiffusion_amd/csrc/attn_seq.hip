@@ -17,10 +17,10 @@
 //   matrix instruction takes it (at most 2^-8 of the mean |v| that the row sees)
 //   O^T += V^T P^T (V^T by ds_read_b64_tr_b16; the S^T registers are the P^T operand)
 // Rows past a tile's last key come from the buffer's range check as zeros. Measured: 64 windows of 16 .. 64
-// rows, 16 heads of 80, 10.2 us (2.5 TB/s); six causal prompts of 70 .. 420, 28 heads over 4, 16.5 us, whose
-// longest block walks 14 tiles of 0.8 us one behind the other; 16 prompts of 400 42 us. Tried and slower or
-// equal: 64-key tiles, three stages with one barrier a tile, 32 rows a wave, two groups of waves a block that
-// share its keys.
+// rows, 16 heads of 80, 10.2 us (2.5 TB/s); six causal prompts of 70 .. 420, 28 heads over 4, 15.2 us, whose
+// longest block walks 14 tiles one behind the other; 16 prompts of 400 46 us, 64 174 (420 TFLOP/s). Tried and
+// slower or equal: 64-key tiles, three stages with one barrier a tile, 32 rows a wave, two groups of waves a
+// block that share its keys, the next tile's scores beside this one's softmax.
 #include <cmath>
 #include <type_traits>
 
@@ -337,15 +337,15 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
 // longest cache that a table can hold (packed sequences: their mean length). Rows are those of one kv
 // head, tokens * G; a group is a (row block, kv head). Times in us, bf16, head_dim 128, 28 heads over 4
 // unless said, the other side in brackets.
-//   few rows (attn_seq_few), 16-row blocks: up to 256 groups with eight waves each (one prompt of 100
-//     tokens 6.6 [9.2 in 64-row blocks]), up to 512 with four, two a CU (one prompt of 200: 8.4 [11.6 with
-//     eight]), and more than that over up to 1500 keys (80 tokens of 24 heads over 24, caches of 20, 300 and 1000:
-//     19, 53 and 176 [32, 69 and 180 with eight; over 8000 1287 with four, 1277 with eight]). 32-row blocks where
-//     16-row ones would be more, or read a long cache again and again (4 new tokens over 20000 keys of 16
-//     sequences: 104 [150]).
-//   64-row blocks (attn_seq): shorter packed sequences (16 prompts of 400: 42 [52 in 256-row blocks]), a short
-//     cache's many rows (16 x 100 new tokens over 300: 20 [25]), and 33 .. 64 rows of a sequence over a long one (16 x
-//     8 new tokens over 20000: 107 [156 in 32-row blocks]).
+//   few rows (attn_seq_few), 16-row blocks: up to 256 groups with eight waves each (one prompt of 100 tokens 7.3
+//     [8.0 in 64-row blocks]), up to 512 with four, two a CU (one prompt of 200: 8.4 [10.9 with eight, 9.3 in 64-row
+//     blocks]), and more than that over up to 1500 keys (80 tokens of 24 heads over 24, caches of 20, 300 and 1000: 17,
+//     49 and 170 [27, 60 and 170 with eight]; over 8000 eight again: 1277 [1287 with four]). 32-row blocks where 16-row
+//     ones would be more, or read a long cache again and again (4 new tokens over 20000 keys of 16 sequences: 135
+//     [189]).
+//   64-row blocks (attn_seq): shorter packed sequences (16 prompts of 400: 46 [53 in 256-row blocks]), a short
+//     cache's many rows (16 x 100 new tokens over 300: 21 [23]), and 33 .. 64 rows of a sequence over a long one (16 x
+//     8 new tokens over 20000: 138 [201 in 32-row blocks]).
 //   256-row blocks (attn_seq_pp) for packed sequences where there are 200 of them, their rounds are full enough, and the
 //     mean length is 700 (10 x 1000: 122 [126 in 64-row blocks]; 5 x 2000: 173 [191]; 1500 where causal heads share
 //     nothing and a block spans 256 tokens: 10 x 1000, 24 heads over 24, 118 [104]). Narrow heads cost them as much as
@@ -390,14 +390,13 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, int head_dim, bo
     p.bm = keys > (head_dim > 64 ? 2048 : 4096) && pad <= (keys > 4096 ? 1.5 : 1.2) ? kPPRows : kBM;
   }
   // Cuts: groups that do not fill the chip share a row's keys, in chunks whose fp32 parts a second kernel
-  // joins: as many as fit 256 CUs at once (1000 new tokens over 5000 keys, two of 40 tiles: 98 [uncut 138, three
-  // chunks 124]; three 64-row work-groups fit a CU), of 8 tiles at least. Up to 1024 keys, none (one token over
-  // 1000: 9.8 in one launch [10.4 in two]). Few rows: 0.6 sqrt(tiles) tiles and 4 at least, where a chunk's time
-  // and the join's meet (one token over 2000, 8000 and 32768 keys: 9.9, 11.6 and 19.5 [11.4, 13.8 and 21.7 with 8 and
+  // joins: as many as fit 256 CUs at once (1000 new tokens over 5000 keys, two of 40 tiles: 99 [uncut 134, three
+  // chunks 120]; three 64-row work-groups fit a CU), of 8 tiles at least. Up to 1024 keys, none (one token over
+  // 800: 8.5 in one launch [9.9 in two]). Few rows: 0.6 sqrt(tiles) tiles and 4 at least, where a chunk's time and
+  // the join's meet (one token over 2000, 8000 and 32768 keys: 9.8, 11.9 and 20.3 [10.9, 13.2 and 21.5 with 8 and
   // 1.4 sqrt(tiles)]). Long tables are cut all the same, so that a long sequence among short ones is shared (48
-  // tokens over 900 .. 32768 keys: 291 [840 uncut]): into 32 tiles (4 and 16 new tokens over 20000 keys of 16
-  // sequences: 104 and 167 [132 and 240 with 64]), 64 where there is one sequence or the groups fill the chip
-  // without a cut.
+  // tokens over 900 .. 32768 keys: 163 [318 uncut]): into 32 tiles (4 new tokens over 20000 keys of 16 sequences: 135
+  // [142 with 64]), 64 where there is one sequence or the groups fill the chip without a cut.
   const double tiles = (double)((table_keys + kKB - 1) / kKB);
   if (tiles <= 16 || (p.bm == kBM && tiles <= 32)) return p;
   const double half = per > 16 ? 0.5 * seqs * kv_heads : 0;  // sequences end inside a block

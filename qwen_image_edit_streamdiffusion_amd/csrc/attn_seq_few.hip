@@ -7,8 +7,8 @@
 // 8 NW .. 16 NW KiB. At the end the waves' (max, sum, O) meet in LDS.
 //
 // Products as in attn_seq.hip (S^T = K Q^T and O^T += V^T P^T on mfma 16x16x32). Measured, 28 heads over 4:
-// 48 single tokens over 900 .. 32768 keys 281 us, 5.7 TB/s, and 5 for the join; 16 over 70 .. 600 8.4 us, 41 new
-// tokens over 309 7.0 (latency: launch, length and table, two or three rounds of tiles, merge).
+// 48 single tokens over 900 .. 32768 keys 281 us, 5.7 TB/s, and 5 for the join; 16 over 70 .. 600 7.9 us, 41 new
+// tokens over 309 6.6 (latency: launch, length and table, two or three rounds of tiles, merge).
 #include "attn_seq.h"
 
 namespace {
