@@ -36,66 +36,90 @@ __device__ __forceinline__ void rfence(T& x) {
 // sees; work-group s of a.shares takes the s-th equal part: the end of one block, whole blocks, the
 // beginning of another. Only the first and the last leave fp32 parts (m, l, O), two slots a work-group,
 // and a second kernel joins them. Lengths are device memory, so the line is laid out here, by every wave.
-constexpr int kShareKeys = 512;  // fewest keys of a share
-constexpr int kBlockKeys = 160;  // what beginning and ending a block costs, in keys
+constexpr int kUnit = 16;              // keys of a unit of the line: sums over all blocks stay in 32 bits (the host sees to it)
+constexpr int kShare = 512 / kUnit;    // fewest units of a share
+constexpr int kBlockKeys = 160;        // what beginning and ending a block costs, in keys
+constexpr int kCut = 1800 / kUnit;     // what cuts cost a call: parts written and read, the join (50 us)
 
 struct Line {  // a block of the line: sequence, its place on the line, the block's ends there
   int b, start, n, kv, nblk, blk;
-  int64_t base, c0, c1;
+  int base, c0, c1;
 };
 // where block x of a sequence begins: the sum of (cost + kept + 256 (i + 1) / G) over the blocks before it
-__device__ __forceinline__ int64_t line_at(const SeqArgs& a, int n, int kv, int x) {
-  return (int64_t)x * (max(kv - n, 0) + kBlockKeys) + (int64_t)((double)((int64_t)(kPPRows / 2) * x * (x + 1)) / a.G);
+__device__ __forceinline__ int line_at(const SeqArgs& a, int n, int kv, int x) {
+  const int64_t keys = (int64_t)x * (max(kv - n, 0) + kBlockKeys) + (int64_t)((double)((int64_t)(kPPRows / 2) * x * (x + 1)) / a.G);
+  return (int)(keys / kUnit);
 }
-__device__ __forceinline__ int64_t uni64(int64_t v) {
-  return (int64_t)(((uint64_t)(uint32_t)uni((int)(v >> 32)) << 32) | (uint32_t)uni((int)v));
-}
-__device__ __forceinline__ int64_t line_of(const SeqArgs& a, int b, int& start, int& n, int& kv) {
-  seq_span<true>(a, b, start, n, kv);
-  return line_at(a, n, kv, (n * a.G + kPPRows - 1) / kPPRows);
-}
-__device__ __forceinline__ int64_t line_length(const SeqArgs& a) {
-  int64_t v = 0;
-  for (int b = threadIdx.x & 63; b < a.B; b += 64) {
-    int start, n, kv;
-    v += line_of(a, b, start, n, kv);
+struct LineSeq {  // a lane's sequence: length on the line, blocks
+  int start, n, kv, nblk, c;
+};
+__device__ __forceinline__ LineSeq line_seq(const SeqArgs& a, int b) {
+  LineSeq s{0, 0, 0, 0, 0};
+  if (b < a.B) {
+    seq_span<true>(a, b, s.start, s.n, s.kv);
+    s.nblk = (s.n * a.G + kPPRows - 1) / kPPRows;
+    s.c = line_at(a, s.n, s.kv, s.nblk);
   }
-#pragma unroll
-  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m, 64);
-  return uni64(v);
+  return s;
+}
+// The line's length and how it is cut: ns equal shares; or, where no block is much longer than a share would
+// be, whole blocks (16 x 100 new tokens over 5000 keys: 150 us, 158 in shares)
+struct Cuts {
+  int total, ns;
+  bool whole;
+};
+__device__ __forceinline__ Cuts line_cuts(const SeqArgs& a, LineSeq& first) {
+  const int lane = threadIdx.x & 63;
+  int v = 0, blocks = 0, longest = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const LineSeq s = line_seq(a, b0 + lane);
+    if (b0 == 0) first = s;
+    v += s.c;
+    blocks += s.nblk;
+    if (s.nblk) longest = max(longest, s.c - line_at(a, s.n, s.kv, s.nblk - 1));
+  }
+  Cuts c;
+  c.total = __builtin_amdgcn_readlane(wave_scan(v), 63);
+  blocks = __builtin_amdgcn_readlane(wave_scan(blocks), 63);
+  longest = (int)wave_max((float)longest);
+  c.ns = min(a.shares, max(1, c.total / kShare));
+  c.whole = blocks <= a.shares && uni(longest) <= c.total / c.ns + kCut;
+  if (c.whole) c.ns = blocks;
+  return c;
 }
 __device__ __forceinline__ void line_block(const SeqArgs& a, Line& l, int x) {
   l.blk = x;
   l.c0 = l.base + line_at(a, l.n, l.kv, x);
   l.c1 = l.base + line_at(a, l.n, l.kv, x + 1);
 }
-// the block that holds position at (< the line's length)
-__device__ __forceinline__ void line_seek(const SeqArgs& a, int64_t at, Line& l) {
+// the block that holds position at (< the line's length), or block number at; first: line_cuts' lanes.
+// false: none, as where offsets overlap and the sums pass 32 bits
+__device__ __forceinline__ bool line_seek(const SeqArgs& a, const LineSeq& first, int at, Line& l, bool number = false) {
   const int lane = threadIdx.x & 63;
-  l.base = 0;
+  l.base = l.nblk = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    int start = 0, n = 0, kv = 0;
-    int64_t c = 0;
-    if (b0 + lane < a.B) c = line_of(a, b0 + lane, start, n, kv);
-    int64_t pre = c;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const int64_t w = __shfl_up(pre, m, 64);
-      if (lane >= m) pre += w;
-    }
+    const LineSeq s = b0 == 0 ? first : line_seq(a, b0 + lane);
+    const int c = number ? s.nblk : s.c, pre = wave_scan(c);
     const unsigned long long hit = __ballot(l.base + pre > at);
     if (hit) {
       const int i = __builtin_ctzll(hit);
       l.b = b0 + i;
-      l.start = __builtin_amdgcn_readlane(start, i);
-      l.n = __builtin_amdgcn_readlane(n, i);
-      l.kv = __builtin_amdgcn_readlane(kv, i);
-      l.base += uni64(__shfl(pre - c, i, 64));
+      l.start = __builtin_amdgcn_readlane(s.start, i);
+      l.n = __builtin_amdgcn_readlane(s.n, i);
+      l.kv = __builtin_amdgcn_readlane(s.kv, i);
+      l.nblk = __builtin_amdgcn_readlane(s.nblk, i);
+      l.base += __builtin_amdgcn_readlane(pre - c, i);
       break;
     }
-    l.base += uni64(__shfl(pre, 63, 64));
+    l.base += __builtin_amdgcn_readlane(pre, 63);
   }
-  l.nblk = (l.n * a.G + kPPRows - 1) / kPPRows;
+  if (l.nblk <= 0) return false;
+  if (number) {
+    const int x = min(max(at - l.base, 0), l.nblk - 1);
+    l.base = 0;
+    line_block(a, l, x);
+    return true;
+  }
   int lo = 0, hi = l.nblk - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -103,6 +127,7 @@ __device__ __forceinline__ void line_seek(const SeqArgs& a, int64_t at, Line& l)
     else hi = mid - 1;
   }
   line_block(a, l, lo);
+  return true;
 }
 __device__ __forceinline__ bool line_next(const SeqArgs& a, Line& l) {
   if (l.blk + 1 < l.nblk) {
@@ -124,23 +149,15 @@ __device__ __forceinline__ int line_tiles(const SeqArgs& a, const Line& l) {
   const int last = (min(l.n * a.G, (l.blk + 1) * kPPRows) - 1) / a.G;
   return (min(l.kv, max(l.kv - l.n + last + 1, 0)) + kKB - 1) / kKB;
 }
-__device__ __forceinline__ int line_tile(const Line& l, int64_t at, int ntot) {
+__device__ __forceinline__ int line_tile(const Line& l, int at, int ntot) {
   if (at <= l.c0) return 0;
   return at >= l.c1 ? ntot : (int)((double)(at - l.c0) * ntot / (double)(l.c1 - l.c0));
 }
-__device__ __forceinline__ int share_count(const SeqArgs& a, int64_t total) {
-  return (int)min((int64_t)a.shares, max((int64_t)1, total / kShareKeys));
-}
 // where share i of ns begins
-__device__ __forceinline__ int64_t share_cut(int64_t total, int ns, int i) { return (int64_t)((double)total * i / ns); }
+__device__ __forceinline__ int share_cut(int total, int ns, int i) { return (int)((double)total * i / ns); }
 // the fp32 part of work-group sh that begins its block (first) or goes on with it
 __device__ __forceinline__ float* share_part(const SeqArgs& a, int sh, bool first, int hk) {
   return a.ws + ((int64_t)(2 * sh + first) * a.Hk + hk) * kPPRows * (a.Dh + 2);
-}
-
-template <typename T>
-__device__ __forceinline__ T* global(T* p) {  // memory of the device, not LDS or scratch
-  return (T*)(__attribute__((address_space(1))) T*)p;
 }
 
 template <bool SHARE, bool PAGED, int KS>  // KS 16-wide steps of the head (4, 6, 8): head_dim <= 16 KS
@@ -153,28 +170,31 @@ __global__ void __launch_bounds__(512) attn_seq_pp_kernel(SeqArgs args) {
   Item it;
   // between two blocks of a share its place waits here: in scalar registers it would push the tiles'
   // addresses out of them
-  __shared__ struct { Line line, head; int64_t end; int head_t0; } place;
+  __shared__ struct { Line line, head; int end, head_t0; } place;
   int t0 = 0;
   bool tail = false;
   if constexpr (SHARE) {
     const SeqArgs& a = args;
     const int sh = blockIdx.x / a.Hk;
-    const int64_t total = line_length(a);
-    const int ns = share_count(a, total);
-    if (sh >= ns) return;
-    const int64_t begin = share_cut(total, ns, sh), end = share_cut(total, ns, sh + 1);
-    if (begin >= end) return;
+    LineSeq first;
+    const Cuts cuts = line_cuts(a, first);
+    if (sh >= cuts.ns) return;
+    int begin = share_cut(cuts.total, cuts.ns, sh), end = share_cut(cuts.total, cuts.ns, sh + 1);
+    if (!cuts.whole && begin >= end) return;
     Line head, line;
-    line_seek(a, begin, head);
+    if (!line_seek(a, first, cuts.whole ? sh : begin, head, cuts.whole)) return;
+    if (cuts.whole) {
+      begin = head.c0;
+      end = head.c1;
+    }
     line = head;
     t0 = line_tile(head, begin, line_tiles(a, head));
     const int head_t0 = t0;
-    if (end < total) {
+    if (!cuts.whole && end < cuts.total) {
       // the beginning of the last block goes first: its tiles and then the first block's are those that the other
       // work-groups of the sequence read at the same time (L2)
       Line l;
-      line_seek(a, end, l);
-      if (l.c0 > begin && line_tile(l, end, line_tiles(a, l)) > 0) {
+      if (line_seek(a, first, end, l) && l.c0 > begin && line_tile(l, end, line_tiles(a, l)) > 0) {
         line = l;
         tail = true;
         t0 = 0;
@@ -202,14 +222,7 @@ __global__ void __launch_bounds__(512) attn_seq_pp_kernel(SeqArgs args) {
     struct { uint32_t w[sizeof(SeqArgs) / 4]; } raw;
 #pragma unroll
     for (unsigned i = 0; i < sizeof(SeqArgs) / 4; ++i) raw.w[i] = p[i];
-    SeqArgs r = __builtin_bit_cast(SeqArgs, raw);
-    r.q = global(r.q);
-    r.out = global(r.out);
-    r.table = global(r.table);
-    r.cu = global(r.cu);
-    r.kv_lens = global(r.kv_lens);
-    r.ws = global(r.ws);
-    return r;
+    return __builtin_bit_cast(SeqArgs, raw);
   };
   const SeqArgs a = fresh();
   const int hk = blockIdx.x % a.Hk;
@@ -530,7 +543,7 @@ __global__ void __launch_bounds__(512) attn_seq_pp_kernel(SeqArgs args) {
   }
   if constexpr (!SHARE) return;
   Line line = place.line;
-  int64_t end = place.end;
+  int end = place.end;
   bool more = true;
   if (tail) {
     end = line.c0;
@@ -557,12 +570,13 @@ __global__ void __launch_bounds__(512) attn_seq_pp_kernel(SeqArgs args) {
 constexpr int kJoinRows = 8, kJoinSplit = kPPRows / (4 * kJoinRows);
 __global__ void __launch_bounds__(256) attn_seq_join_shares_kernel(SeqArgs a) {
   const int hk = blockIdx.x % a.Hk, u = blockIdx.x / a.Hk, s = 1 + u / kJoinSplit;
-  const int64_t total = line_length(a);
-  const int ns = share_count(a, total);
-  if (s >= ns) return;
-  auto cut = [&](int i) { return share_cut(total, ns, i); };
+  LineSeq first;
+  const Cuts cuts = line_cuts(a, first);
+  const int ns = cuts.ns;
+  if (cuts.whole || s >= ns) return;
+  auto cut = [&](int i) { return share_cut(cuts.total, ns, i); };
   Line l;
-  line_seek(a, cut(s), l);
+  if (!line_seek(a, first, cut(s), l)) return;
   const int ntot = line_tiles(a, l), t = line_tile(l, cut(s), ntot);
   if (t == 0 || t == ntot || line_tile(l, cut(s - 1), ntot) > 0) return;
   const int lane = threadIdx.x & 63, d = 2 * lane < a.Dh ? 2 * lane : 0;

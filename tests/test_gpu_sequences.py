@@ -339,7 +339,9 @@ PAGED = [([1], [1], 1, 1, 64, 16, "heads"), ([1, 1, 1], [5, 700, 64], 28, 4, 128
          ([400, 5, 0, 360], [4500, 900, 40, 380], 16, 2, 128, 64, "heads"), ([400, 380], [4500, 4200], 14, 2, 72, 16, "rows"),
          ([900, 300, 1], [5000, 0, 4000], 16, 2, 64, 32, "heads"), ([1000, 40], [1000, 4300], 16, 2, 128, 64, "heads"),
          ([800], [4800], 20, 1, 128, 16, "rows"), ([10] * 70, [70] * 69 + [4200], 64, 1, 64, 16, "heads"),
-         ([900, 700], [20, 5000], 24, 3, 96, 128, "heads")]
+         ([900, 700], [20, 5000], 24, 3, 96, 128, "heads"),
+         # of one length: whole blocks
+         ([500] * 2, [4300] * 2, 24, 4, 128, 64, "heads"), ([400] * 3, [4200] * 3, 16, 4, 64, 64, "rows")]
 
 
 @pytest.mark.parametrize("new,kv,H,Hk,Dh,P,layout", PAGED)
