@@ -434,6 +434,50 @@ def test_attention_paged_bad_pages_read_as_zeros():
     _check(full, want, tol)
 
 
+@pytest.mark.parametrize("new,kv,H,Hk", [([2, 1], [70, 40], 4, 2), ([50, 60], [900, 300], 28, 4), ([200, 90], [1500, 100], 28, 4),
+                                         ([500, 400], [4400, 600], 28, 4), ([900, 700], [2300, 800], 28, 4)])
+def test_attention_paged_bad_offsets_and_lengths_stay_inside(new, kv, H, Hk):
+    """Offsets outside the rows are clamped, a negative length is an empty cache: rows that see nothing are 0."""
+    ops = _ops()
+    q, ks, vs, kp, vp, table = _paged(_gen(31), new, kv, H, Hk, 128, 64)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    want, tol = paged_ref(q, ks, vs, new, kv)
+    got = ops.attention_paged(q.to(DEV), kp, vp, table.to(DEV), i32([kv[0], -3]), cu_seqlens=i32([-7, new[0], 2 ** 31 - 1]))
+    _check(got[:new[0]], want[:new[0]], tol[:new[0]])
+    assert not got[new[0]:].any()
+    # descending offsets: an empty sequence, then all rows
+    got = ops.attention_paged(q.to(DEV), kp, vp, table.to(DEV), i32([5, kv[1]]), cu_seqlens=i32([sum(new), 0, sum(new)]))
+    only = slice(sum(new) - new[1], None)
+    _check(got[only], want[only], tol[only])
+
+
+def test_captured_chunk_replays():
+    """Many rows over a long table in a graph: replays with other offsets, lengths and q in the same buffers."""
+    ops = _ops()
+    new, kv, H, Hk, Dh, P = [500, 300, 100], [4500, 3000, 100], 28, 4, 128, 64
+    q, ks, vs, kp, vp, table = _paged(_gen(32), new, kv, H, Hk, Dh, P)
+    qd, td = q.to(DEV), table.to(DEV)
+    cu, lens = _cu(new).to(DEV), torch.tensor(kv, dtype=torch.int32, device=DEV)
+    ws = torch.empty(ops.attention_paged_workspace_bytes(len(q), 3, H, Hk, Dh, table.shape[1], P), dtype=torch.uint8, device=DEV)
+    out = torch.zeros_like(qd)
+    run = lambda o, w: ops.attention_paged(qd, kp, vp, td, lens, cu_seqlens=cu, out=o, workspace=w)  # noqa: E731
+    run(out, ws)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        run(out, ws)
+    for n, k in ((new, kv), ([100, 700, 100], [4500, 3000, 70]), ([900, 0, 0], [4000, 1, 0]), ([1, 1, 1], [3, 2, 1])):
+        cu.copy_(_cu(n))
+        lens.copy_(torch.tensor(k, dtype=torch.int32))
+        qd.neg_()
+        ref = torch.zeros_like(qd)
+        run(ref, None)
+        out.zero_()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref) and torch.isfinite(out).all()
+
+
 def test_attention_paged_offsets_past_32_bits():
     """A pool of more than 2^31 elements: its last pages."""
     ops = _ops()
