@@ -124,3 +124,18 @@ class PagedKVCache:
         table = [self._seqs[s].pages + [0] * (width - len(self._seqs[s].pages)) for s in seqs]
         i32 = lambda v: torch.tensor(v, dtype=torch.int32).to(self.device)  # noqa: E731
         return CacheStep(i32(table), i32(lens), i32(cu), torch.tensor(slots, dtype=torch.int64).to(self.device))
+
+    def take_back(self, seqs: Sequence[int], new: Sequence[int]) -> None:
+        """Undo the last ``step`` of these sequences, as where its forward failed: the tokens are no longer
+        counted, the pages that only they needed are free. Not once the sequences were forked behind it."""
+        steps = [(self._seqs[seq], n) for seq, n in zip(seqs, new)]
+        keep = [-(-(s.length - n) // self.page_size) for s, n in steps]
+        if any(not 0 <= n <= s.length for s, n in steps):
+            raise ValueError("more tokens than the sequence has")
+        if any(self._users[p] != 1 for (s, _), k in zip(steps, keep) for p in s.pages[k:]):
+            raise ValueError("pages that another sequence shares")
+        for (s, n), k in zip(reversed(steps), reversed(keep)):  # the free pages in their order before the step
+            self._free += reversed(s.pages[k:])
+            for p in s.pages[k:]:
+                self._users[p] = 0
+            s.pages, s.length = s.pages[:k], s.length - n

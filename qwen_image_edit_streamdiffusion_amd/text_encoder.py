@@ -298,15 +298,19 @@ class QwenVLTextModel:
         st = cache.step(seqs, lens)
         c = self.config
         H, Hk, Dh = c.num_attention_heads, c.num_key_value_heads, c.head_dim
-        nb = ops.attention_paged_workspace_bytes(sum(lens), len(lens), H, Hk, Dh, st.page_table.shape[1], cache.page_size)
-        ws = torch.empty(nb, dtype=torch.uint8, device=self.device) if nb else None
+        try:
+            nb = ops.attention_paged_workspace_bytes(sum(lens), len(lens), H, Hk, Dh, st.page_table.shape[1], cache.page_size)
+            ws = torch.empty(nb, dtype=torch.uint8, device=self.device) if nb else None
 
-        def attend(layer, qkv, q3, pos, out):
-            k, v = cache.k[layer], cache.v[layer]
-            ops.rope_append(qkv, H, Hk, Dh, pos, self.turns, self.axis, k, v, st.slots)
-            ops.attention_paged(q3, k, v, st.page_table, st.kv_lens, cu_seqlens=st.cu_seqlens, out=out, workspace=ws)
+            def attend(layer, qkv, q3, pos, out):
+                k, v = cache.k[layer], cache.v[layer]
+                ops.rope_append(qkv, H, Hk, Dh, pos, self.turns, self.axis, k, v, st.slots)
+                ops.attention_paged(q3, k, v, st.page_table, st.kv_lens, cu_seqlens=st.cu_seqlens, out=out, workspace=ws)
 
-        return list(self._rows(tokens, position_ids, lens, attend).split(lens))
+            return list(self._rows(tokens, position_ids, lens, attend).split(lens))
+        except Exception:
+            cache.take_back(seqs, lens)  # their k / v may be missing
+            raise
 
     def _check_positions(self, position_ids, lens):
         if not self.layers:
@@ -497,7 +501,7 @@ class QwenVLEncoder:
         if best is not None:
             self.prefixes.move_to_end(best)
             if common == S:
-                return self.prefixes[best].hidden[:S]
+                return self.prefixes[best].hidden[:S].clone()  # the caller's own: what is kept stays as it is
         pos = self._positions(ids, pixel_values, image_grid_thw)
         if image.numel() and int(image[-1]) >= common:
             new = self._embeds(ids, pixel_values, image_grid_thw)[0][common:]
@@ -525,7 +529,7 @@ class QwenVLEncoder:
         while len(self.prefixes) > self.prefix_cache_size:
             old, _ = self.prefixes.popitem(last=False)
             self.kv.drop(old)
-        return hidden
+        return hidden.clone()
 
     def _vision_key(self, pixel_values: torch.Tensor, image_grid_thw):
         """(grid and content digest, grid) of a prompt's pictures."""

@@ -81,6 +81,10 @@ def test_extend_over_the_cache_vs_transformers():
     more = torch.randint(0, 1000, (3,), generator=g)
     with pytest.raises(ValueError):  # a refused call leaves the sequence as it was
         te.extend(cache, [seqs[0]], [more], [torch.zeros(3, 4, dtype=torch.long)])
+    lin, te.lin = te.lin, None  # a forward that fails on its way does, too
+    with pytest.raises(AttributeError):
+        te.extend(cache, [seqs[0]], [more])
+    te.lin = lin
     got = te.extend(cache, [seqs[0]], [more])[0]
     assert _rel(got, VL.text_forward(m, input_ids=torch.cat([ids[0], more]))[150:]) <= 2e-2
 
@@ -149,6 +153,7 @@ def test_prefix_cache_vs_transformers():
         got = enc(ids, x, grid)
         want = VL.vl_forward(m, ids, x, grid)[0]
         assert got.shape == want.shape and _rel(got, want) <= 2e-2
+        got.zero_()  # the caller's own rows: what is kept stays as it is
         new = sum(ran[before:])
         if rows == 0:
             assert new == 0

@@ -141,6 +141,24 @@ def test_paged_cache_steps_and_pages():
         c.length(a)
 
 
+def test_paged_cache_takes_a_step_back():
+    c = _cache()
+    a, b = c.add(), c.add()
+    c.step([a, b], [20, 16])
+    before = c.free_pages, list(c._free)
+    st = c.step([a, b], [40, 3])
+    c.take_back([a, b], [40, 3])
+    assert (c.free_pages, c.length(a), c.length(b)) == (before[0], 20, 16)
+    again = c.step([a, b], [40, 3])
+    assert again.slots.tolist() == st.slots.tolist() and again.page_table.tolist() == st.page_table.tolist()
+    with pytest.raises(ValueError):
+        c.take_back([b], [20])
+    c.fork(a, 48)  # a's third page is shared now
+    with pytest.raises(ValueError):
+        c.take_back([a], [40])
+    assert c.length(a) == 60
+
+
 def test_paged_cache_shared_pages_and_refusals():
     from qwen_image_edit_streamdiffusion_amd.kv_cache import CacheFull, PagedKVCache
     c = _cache(4)
