@@ -340,10 +340,12 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
 //   few rows (attn_seq_few), 16-row blocks: up to 256 groups with eight waves each (one prompt of 100 tokens 7.3
 //     [8.0 in 64-row blocks]), up to 512 with four, two a CU (one prompt of 200: 8.4 [10.9 with eight, 9.3 in 64-row
 //     blocks]), and more than that over up to 1500 keys (80 tokens of 24 heads over 24, caches of 20, 300 and 1000: 17,
-//     49 and 170 [27, 60 and 170 with eight]; over 8000 eight again: 1277 [1287 with four]). 32-row blocks where 16-row
-//     ones would be more, or read a long cache again and again (4 new tokens over 20000 keys of 16 sequences: 135
-//     [189]).
-//   64-row blocks (attn_seq): shorter packed sequences (16 prompts of 400: 46 [53 in 256-row blocks]), a short
+//     49 and 170 [27, 60 and 170 with eight]; over 8000 eight again: 1277 [1287 with four]). 32-row blocks over more
+//     than 256 keys where 16-row ones would be more than 256 (200 new tokens over 1000: 14.4 [17.0]; 10 x 20 over 300,
+//     16 heads of 80, 8.6 [10.1]), or read a long cache again and again (4 new tokens over 20000 keys of 16 sequences:
+//     135 [189]).
+//   64-row blocks (attn_seq): shorter packed sequences (16 prompts of 400: 46 [53 in 256-row blocks]; from 200 groups
+//     on very short ones, 16 x 30, 16 heads of 80: 5.6 [7.0 in 16-row blocks]), a short
 //     cache's many rows (16 x 100 new tokens over 300: 21 [23]), and 33 .. 64 rows of a sequence over a long one (16 x
 //     8 new tokens over 20000: 138 [201 in 32-row blocks]).
 //   256-row blocks (attn_seq_pp) for packed sequences where there are 200 of them, their rounds are full enough, and the
@@ -364,7 +366,8 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, int head_dim, bo
   const double keys = paged ? (double)table_keys : (double)tokens / seqs;
   const double g16 = kv_heads * fmax(seqs, rows / 16), g32 = kv_heads * fmax(seqs, rows / 32),
                g64 = kv_heads * fmax(seqs, rows / kBM), g256 = kv_heads * fmax(1.0, rows / kPPRows);
-  const int few16 = g16 <= 256 ? 8 : 4;
+  const double r16 = (double)kv_heads * seqs * ceil(per / 16), r32 = (double)kv_heads * seqs * ceil(per / 32);  // as rounded
+  const int few16 = r16 <= 256 ? 8 : 4;
   // from what length on 256-row blocks pay, and how full their rounds of 256 are
   const double longest = head_dim > 96  ? (causal && heads == kv_heads ? 1500 : 700)
                          : head_dim > 64 ? (causal ? 1800 : 1000)
@@ -372,7 +375,7 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, int head_dim, bo
   const double rounds = ceil(g256 / 256), pad = ceil(per / kPPRows) * kPPRows / per;
   SeqPlan p{kBM, few16, 0, 1, 0};
   if (!paged) {
-    if (g16 <= 512) p.bm = 16;
+    if (g16 <= 512 && !(keys <= 100 && g16 >= 200)) p.bm = 16;
     else if (keys >= longest && g256 >= 200 && (g256 >= 512 || g256 >= 0.65 * 256 * rounds)) p.bm = kPPRows;
     return p;
   }
@@ -380,11 +383,12 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, int head_dim, bo
     p.bm = 16;
     p.waves = keys <= 1536 ? few16 : 8;
   } else if (keys <= 512) {
-    p.bm = g16 <= 512 ? 16 : kBM;
+    p.bm = r16 <= 256 ? 16 : r32 <= 256 && keys > 256 ? 32 : g16 <= 512 ? 16 : kBM;
+    if (p.bm == 32) p.waves = 8;
   } else if (per > 32 && per <= 64 && g32 * keys > 3e5) {
     p.bm = kBM;
   } else if (per <= 32 || (g32 <= 512 && g32 * keys <= 1.5e6)) {
-    p.bm = g16 <= 512 && g16 * keys <= 4e5 ? 16 : 32;
+    p.bm = r16 <= 256 && g16 * keys <= 4e5 ? 16 : 32;
     if (p.bm == 32) p.waves = 8;
   } else {
     p.bm = keys > (head_dim > 64 ? 2048 : 4096) && pad <= (keys > 4096 ? 1.5 : 1.2) ? kPPRows : kBM;
