@@ -218,7 +218,8 @@ def _split(xd, H, Hk, Dh):
 PACKED = [([1], 1, 1, 64), ([0, 5, 0, 64, 65, 0], 4, 2, 64), ([63, 1, 128, 200], 28, 4, 128), ([700], 6, 2, 128),
           ([33, 100], 16, 16, 80), ([129], 28, 1, 72), ([257, 64], 3, 3, 8), ([90, 400, 31], 16, 2, 96),
           ([1] * 70 + [3], 7, 1, 40), ([1100, 2], 8, 8, 128), ([513, 1, 300], 20, 1, 128), ([100], 28, 4, 128),
-          ([2600, 1500], 16, 2, 128), ([2600, 1500], 16, 2, 72), ([2600, 1500], 16, 2, 64)]  # the last: 256-row blocks
+          ([2600, 1500], 16, 2, 128), ([2600, 1500], 16, 2, 72), ([2600, 1500], 16, 2, 64),
+          ([3000, 2500], 16, 2, 128), ([3000, 2500], 16, 2, 72), ([3600], 16, 2, 64), ([30] * 16, 16, 16, 80)]  # 256-row blocks
 
 
 @pytest.mark.parametrize("causal", [True, False])
@@ -340,6 +341,12 @@ PAGED = [([1], [1], 1, 1, 64, 16, "heads"), ([1, 1, 1], [5, 700, 64], 28, 4, 128
          ([900, 300, 1], [5000, 0, 4000], 16, 2, 64, 32, "heads"), ([1000, 40], [1000, 4300], 16, 2, 128, 64, "heads"),
          ([800], [4800], 20, 1, 128, 16, "rows"), ([10] * 70, [70] * 69 + [4200], 64, 1, 64, 16, "heads"),
          ([900, 700], [20, 5000], 24, 3, 96, 128, "heads"),
+         # 256-row blocks uncut and in chunks, 64-row ones in chunks, 32-row ones, four waves
+         ([2200], [2300], 28, 4, 128, 64, "heads"), ([3600], [3700], 16, 2, 80, 64, "rows"), ([4200], [4300], 16, 2, 64, 16, "heads"),
+         ([700, 900], [700, 3000], 16, 2, 128, 16, "heads"), ([60] * 6, [3000] * 5 + [100], 16, 16, 64, 32, "heads"),
+         ([60] * 6, [3000] * 5 + [100], 16, 16, 80, 64, "rows"), ([600] * 3, [600, 610, 900], 16, 16, 80, 64, "heads"),
+         ([200], [1000], 28, 4, 64, 64, "heads"), ([1] * 70, [40] * 69 + [700], 16, 16, 64, 64, "heads"),
+         ([1] * 70, [40] * 69 + [700], 16, 16, 80, 16, "rows"), ([2] * 70, [45] * 69 + [700], 16, 16, 128, 64, "heads"),
          # of one length: whole blocks
          ([500] * 2, [4300] * 2, 24, 4, 128, 64, "heads"), ([400] * 3, [4200] * 3, 16, 4, 64, 64, "rows")]
 
