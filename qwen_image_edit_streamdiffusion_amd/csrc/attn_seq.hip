@@ -17,7 +17,7 @@
 //   matrix instruction takes it (at most 2^-8 of the mean |v| that the row sees)
 //   O^T += V^T P^T (V^T by ds_read_b64_tr_b16; the S^T registers are the P^T operand)
 // Rows past a tile's last key come from the buffer's range check as zeros. Measured: 64 windows of 16 .. 64
-// rows, 16 heads of 80, 10.2 us (2.5 TB/s); six causal prompts of 70 .. 420, 28 heads over 4, 15.2 us, whose
+// rows, 16 heads of 80, 10.2 us (2.5 TB/s); six causal prompts of 70 .. 420, 28 heads over 4, 14.9 us, whose
 // longest block walks 14 tiles one behind the other; 16 prompts of 400 46 us, 64 174 (420 TFLOP/s). Tried and
 // slower or equal: 64-key tiles, three stages with one barrier a tile, 32 rows a wave, two groups of waves a
 // block that share its keys, the next tile's scores beside this one's softmax.
