@@ -128,11 +128,14 @@ class PagedKVCache:
     def take_back(self, seqs: Sequence[int], new: Sequence[int]) -> None:
         """Undo the last ``step`` of these sequences, as where its forward failed: the tokens are no longer
         counted, the pages that only they needed are free. Not once the sequences were forked behind it."""
+        if len(seqs) != len(new) or len(set(seqs)) != len(seqs):
+            raise ValueError("one count of tokens for each of distinct sequences")
         steps = [(self._seqs[seq], n) for seq, n in zip(seqs, new)]
         keep = [-(-(s.length - n) // self.page_size) for s, n in steps]
         if any(not 0 <= n <= s.length for s, n in steps):
             raise ValueError("more tokens than the sequence has")
-        if any(self._users[p] != 1 for (s, _), k in zip(steps, keep) for p in s.pages[k:]):
+        # the pages that hold such tokens, a part of the first one's slots may stay
+        if any(self._users[p] != 1 for s, n in steps if n for p in s.pages[(s.length - n) // self.page_size:]):
             raise ValueError("pages that another sequence shares")
         for (s, n), k in zip(reversed(steps), reversed(keep)):  # the free pages in their order before the step
             self._free += reversed(s.pages[k:])

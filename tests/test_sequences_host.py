@@ -180,3 +180,22 @@ def test_paged_cache_shared_pages_and_refusals():
                 lambda: PagedKVCache(1, 1, 64, 4, 24, "cpu"), lambda: PagedKVCache(1, 1, 60, 4, 16, "cpu")):
         with pytest.raises((ValueError, KeyError)):
             bad()
+
+
+def test_paged_cache_takes_back_only_tokens_of_its_own():
+    c = _cache()
+    a, b = c.add(), c.add()
+    c.step([a, b], [28, 5])
+    c.step([a], [4])  # a's second page fills up to its end
+    f = c.fork(a, 32)  # and is shared
+    state = lambda: (c.free_pages, c.length(a), c.length(b), c.length(f))  # noqa: E731
+    before = state()
+    for bad in (([a], [4]), ([a], [1]), ([b, b], [2, 2]), ([b], [2, 2]), ([b], [-1])):
+        with pytest.raises(ValueError):
+            c.take_back(*bad)
+        assert state() == before, bad  # a refused one changes nothing
+    c.take_back([a, b], [0, 5])  # no token of a
+    assert (c.length(a), c.length(b), c.free_pages) == (32, 0, 6)
+    c.step([f], [3])
+    c.take_back([f], [3])  # tokens behind the shared pages
+    assert (c.length(f), c.free_pages) == (32, 6)
