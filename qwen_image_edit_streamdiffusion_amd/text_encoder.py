@@ -525,7 +525,7 @@ class QwenVLEncoder:
             raise
         if common:
             hidden = torch.cat([self.prefixes[best].hidden[:common], hidden])
-        self.prefixes[seq] = _Prefix(ids, key, hidden)
+        self.prefixes[seq] = _Prefix(ids.clone(), key, hidden)  # the caller may use its buffer again
         while len(self.prefixes) > self.prefix_cache_size:
             old, _ = self.prefixes.popitem(last=False)
             self.kv.drop(old)
