@@ -436,6 +436,7 @@ class QwenVLEncoder:
 
     def load_state_dict(self, sd: Dict[str, torch.Tensor]) -> "QwenVLEncoder":
         self.clear_prefixes()
+        self.vision_cache.clear()
         self.text.load_state_dict({k: v for k, v in sd.items() if "visual." not in k})
         self.vision.load_state_dict({k: v for k, v in sd.items() if "visual." in k})
         return self

@@ -93,3 +93,17 @@ def test_the_callers_ids_may_change_after_the_call(encoder):
     assert _ask(enc, ids) == [70]
     ids[0] = (ids[0] + 1) % 190
     assert _ask(enc, ids) == [120]
+
+
+def test_other_weights_forget_what_the_old_ones_gave(encoder):
+    """Kept prompts and kept pictures both."""
+    enc = encoder(2)
+    enc.vision.load_state_dict = lambda sd: enc.vision
+    enc.vision.forward = lambda pv, grid: torch.full((4, 256), float(len(seen)))
+    seen, pv, grid = [], torch.zeros(16, 1176), [(1, 4, 4)]
+    assert _ask(enc, _ids(80, 3)) == [80] and enc._vision(pv, grid)[0, 0] == 0
+    seen.append(1)
+    assert enc._vision(pv, grid)[0, 0] == 0  # the same picture
+    enc.load_state_dict({})
+    assert enc._vision(pv, grid)[0, 0] == 1
+    assert _ask(enc, _ids(80, 3)) == [80]
