@@ -488,8 +488,14 @@ class QwenVLEncoder:
     def _forward_prefix(self, ids: torch.Tensor, pixel_values, image_grid_thw) -> torch.Tensor:
         ids = ids.cpu()
         S = ids.numel()
-        key = None if pixel_values is None else self._vision_key(pixel_values, image_grid_thw)[0]
+        key, rows = None, 0
         image = (ids == self.image_token_id).nonzero().view(-1)
+        if pixel_values is not None:
+            key, grid = self._vision_key(pixel_values, image_grid_thw)
+            rows = sum(t * h * w for t, h, w in grid) // self.vision.config.spatial_merge_size ** 2
+        pos = self._positions(ids, pixel_values, image_grid_thw)
+        if image.numel() != rows:  # as for a prompt that runs whole, however much of this one is kept
+            raise ValueError(f"{image.numel()} image tokens but {rows} image embeddings")
         best, common = None, 0
         for seq, p in reversed(self.prefixes.items()):  # of equals, the one used last
             m = min(S, p.ids.numel())
@@ -503,7 +509,6 @@ class QwenVLEncoder:
             self.prefixes.move_to_end(best)
             if common == S:
                 return self.prefixes[best].hidden[:S].clone()  # the caller's own: what is kept stays as it is
-        pos = self._positions(ids, pixel_values, image_grid_thw)
         if image.numel() and int(image[-1]) >= common:
             new = self._embeds(ids, pixel_values, image_grid_thw)[0][common:]
         else:

@@ -107,3 +107,27 @@ def test_other_weights_forget_what_the_old_ones_gave(encoder):
     enc.load_state_dict({})
     assert enc._vision(pv, grid)[0, 0] == 1
     assert _ask(enc, _ids(80, 3)) == [80]
+
+
+def _picture(value, grid):
+    return torch.full((sum(t * h * w for t, h, w in grid), 1176), value), grid
+
+
+def test_pictures_are_counted_for_a_kept_prompt_too(encoder):
+    """A prompt that lacks a picture's tokens is refused, whatever part of it is kept."""
+    enc = encoder(4)
+    grid = [(1, 4, 4), (1, 8, 4)]  # 4 and 8 tokens
+    pv = _picture(1.0, grid)
+    run = lambda n: torch.full((n,), IMAGE)  # noqa: E731
+    a, b = _ids(70, 4), _ids(30, 5)
+    whole = torch.cat([a, run(4), b, run(8), b])
+    assert _ask(enc, whole, *pv) == [len(whole)]
+    for ids in (whole[:len(a) + 4 + 5], torch.cat([whole[:len(a) + 4], _ids(9, 6)]), whole[:60], whole[:len(a) + 2],
+                whole[:len(a) + 4 + len(b) + 3]):
+        with pytest.raises(ValueError):
+            enc(ids, *pv)
+    with pytest.raises(ValueError):  # image tokens without a picture
+        enc(whole, None, None)
+    assert _ask(enc, whole, *pv) == [] and _ask(enc, torch.cat([whole[:-3], _ids(9, 6)]), *pv) == [9]
+    # other pictures of the same sizes: the text before the first one is shared
+    assert _ask(enc, whole, *_picture(2.0, grid)) == [len(whole) - len(a)]
