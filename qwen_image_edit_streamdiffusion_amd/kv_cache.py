@@ -61,6 +61,10 @@ class PagedKVCache:
     def length(self, seq: int) -> int:
         return self._seqs[seq].length
 
+    def held_pages(self, seq: int) -> int:
+        """Pages that hold a sequence's tokens, those that it shares among them."""
+        return len(self._seqs[seq].pages)
+
     def add(self) -> int:
         """A new, empty sequence."""
         self._next += 1

@@ -509,20 +509,26 @@ class QwenVLEncoder:
             self.prefixes.move_to_end(best)
             if common == S:
                 return self.prefixes[best].hidden[:S].clone()  # the caller's own: what is kept stays as it is
+        if self.kv is None:
+            self.kv = self.text.new_cache(self.prefix_pages)
+        kv = self.kv
+        # room for the new sequence's pages beside the shared ones; where even all others' would not do, the prompt
+        # it begins like goes and it runs whole
+        whole = -(-S // kv.page_size)
+        need = whole - common // kv.page_size
+        if best is not None and kv.num_pages - kv.held_pages(best) < need and whole <= kv.num_pages:
+            kv.drop(best)
+            del self.prefixes[best]
+            best, common, need = None, 0, whole
+        while whole <= kv.num_pages and kv.free_pages < need and self.prefixes and next(iter(self.prefixes)) != best:
+            old, _ = self.prefixes.popitem(last=False)  # the one used longest ago first
+            kv.drop(old)
+        if kv.free_pages < need:  # longer than the pool: not kept, and those that are stay
+            return self.text.forward_packed([self._embeds(ids, pixel_values, image_grid_thw)[0]], [pos])[0]
         if image.numel() and int(image[-1]) >= common:
             new = self._embeds(ids, pixel_values, image_grid_thw)[0][common:]
         else:
             new = ids[common:]  # every image row lies in what is shared
-        if self.kv is None:
-            self.kv = self.text.new_cache(self.prefix_pages)
-        # room: the new sequence's pages beside the shared ones, older prompts go first
-        need = -(-S // self.kv.page_size) - common // self.kv.page_size
-        while self.kv.free_pages < need and self.prefixes and next(iter(self.prefixes)) != best:
-            old, _ = self.prefixes.popitem(last=False)
-            self.kv.drop(old)
-        if self.kv.free_pages < need:
-            emb = self._embeds(ids, pixel_values, image_grid_thw)[0]
-            return self.text.forward_packed([emb], [pos])[0]  # longer than the cache: not kept
         seq = self.kv.fork(best, common) if common else self.kv.add()
         try:
             hidden = self.text.extend(self.kv, [seq], [new], [pos[:, common:]])[0]

@@ -131,3 +131,38 @@ def test_pictures_are_counted_for_a_kept_prompt_too(encoder):
     assert _ask(enc, whole, *pv) == [] and _ask(enc, torch.cat([whole[:-3], _ids(9, 6)]), *pv) == [9]
     # other pictures of the same sizes: the text before the first one is shared
     assert _ask(enc, whole, *_picture(2.0, grid)) == [len(whole) - len(a)]
+
+
+def test_a_prompt_that_does_not_fit_beside_what_it_shares_is_kept_instead(encoder):
+    """Two prompts of more than half the pool that begin alike: the second one runs whole once, then it is kept."""
+    enc = encoder(1)
+    a = _ids(1100, 7)
+    b = torch.cat([a[:70], _ids(1030, 8)])
+    common = int((a != b).nonzero()[0])
+    assert enc.prefix_pages == 32 and _ask(enc, a) == [1100] and common >= 70
+    assert _ask(enc, b) == [1100]
+    assert _ask(enc, b) == [] and _ask(enc, b) == [] and enc.kv.free_pages == 32 - 18
+    c = torch.cat([a[:70], _ids(50, 9)])  # beside it there is room for this one
+    assert _ask(enc, c) in ([120 - n] for n in range(70, 74))
+
+
+def test_kept_prompts_beside_it_stay_where_they_fit(encoder):
+    """Of three kept prompts only the one that blocks a longer one goes."""
+    enc = encoder(4, pages=32)
+    small, other, a = _ids(100, 10), _ids(120, 11), _ids(1100, 12)
+    assert [_ask(enc, x) for x in (small, other, a)] == [[100], [120], [1100]]
+    b = torch.cat([a[:70], _ids(1400, 13)])  # 23 pages: 22 beside a's 18 never fit, 23 beside the two others do
+    assert _ask(enc, b) == [1470]
+    assert _ask(enc, small) == _ask(enc, other) == _ask(enc, b) == [] and len(enc.prefixes) == 3
+
+
+def test_a_prompt_longer_than_the_pool_leaves_the_kept_ones(encoder):
+    enc = encoder(4)
+    kept = [_ids(200 + i, 20 + i) for i in range(4)]
+    for x in kept:
+        _ask(enc, x)
+    free = enc.kv.free_pages
+    for long in (_ids(6000, 30), torch.cat([kept[1][:150], _ids(6000, 31)])):
+        assert _ask(enc, long) == [len(long)]
+        assert enc.kv.free_pages == free and len(enc.prefixes) == 4
+    assert [_ask(enc, x) for x in kept] == [[]] * 4
