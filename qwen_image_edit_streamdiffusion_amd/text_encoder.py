@@ -532,16 +532,17 @@ class QwenVLEncoder:
         seq = self.kv.fork(best, common) if common else self.kv.add()
         try:
             hidden = self.text.extend(self.kv, [seq], [new], [pos[:, common:]])[0]
+            if common:
+                hidden = torch.cat([self.prefixes[best].hidden[:common], hidden])
+            own = hidden.clone()  # the caller's; what is kept stays as it is
         except Exception:
             self.kv.drop(seq)
             raise
-        if common:
-            hidden = torch.cat([self.prefixes[best].hidden[:common], hidden])
         self.prefixes[seq] = _Prefix(ids.clone(), key, hidden)  # the caller may use its buffer again
         while len(self.prefixes) > self.prefix_cache_size:
             old, _ = self.prefixes.popitem(last=False)
             self.kv.drop(old)
-        return hidden.clone()
+        return own
 
     def _vision_key(self, pixel_values: torch.Tensor, image_grid_thw):
         """(grid and content digest, grid) of a prompt's pictures."""

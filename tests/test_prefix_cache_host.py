@@ -166,3 +166,18 @@ def test_a_prompt_longer_than_the_pool_leaves_the_kept_ones(encoder):
         assert _ask(enc, long) == [len(long)]
         assert enc.kv.free_pages == free and len(enc.prefixes) == 4
     assert [_ask(enc, x) for x in kept] == [[]] * 4
+
+
+def test_a_call_that_fails_at_its_end_holds_no_pages(encoder):
+    """What is shared and the new rows no longer fit into memory together: the new sequence goes."""
+    enc = encoder(2)
+    a = _ids(300, 40)
+    b = torch.cat([a[:192], _ids(100, 41)])
+    assert _ask(enc, a) == [300]
+    free, kept = enc.kv.free_pages, next(iter(enc.prefixes.values()))
+    hidden, kept.hidden = kept.hidden, kept.hidden[:, :2]  # rows that do not go with the new ones
+    with pytest.raises(RuntimeError):
+        enc(b)
+    assert enc.kv.free_pages == free and len(enc.prefixes) == 1
+    kept.hidden = hidden
+    assert _ask(enc, b) in ([100], [99], [98]) and _ask(enc, a) == []
