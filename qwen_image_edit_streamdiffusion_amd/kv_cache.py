@@ -79,6 +79,12 @@ class PagedKVCache:
             self._users[p] = 1
         return got
 
+    def _give(self, pages: Sequence[int]) -> None:
+        for p in pages:
+            self._users[p] -= 1
+            if not self._users[p]:
+                self._free.append(p)
+
     def fork(self, seq: int, length: int) -> int:
         """A new sequence that begins with the first ``length`` tokens of ``seq``: whole pages are
         shared, a page that ends behind them is copied."""
@@ -87,21 +93,22 @@ class PagedKVCache:
             raise ValueError(f"{length} of {src.length} tokens")
         whole, rest = divmod(length, self.page_size)
         own = self._take(1) if rest else []
+        if rest:
+            try:
+                for t in (self.k, self.v):
+                    ops.copy_batched(t[:, src.pages[whole]], t[:, own[0]])
+            except BaseException:
+                self._give(own)
+                raise
         for p in src.pages[:whole]:
             self._users[p] += 1
-        if rest:
-            for t in (self.k, self.v):
-                ops.copy_batched(t[:, src.pages[whole]], t[:, own[0]])
         new = self.add()
         self._seqs[new] = _Sequence(src.pages[:whole] + own, length)
         return new
 
     def drop(self, seq: int) -> None:
         """Give a sequence's pages back (shared ones when their last user goes)."""
-        for p in self._seqs.pop(seq).pages:
-            self._users[p] -= 1
-            if not self._users[p]:
-                self._free.append(p)
+        self._give(self._seqs.pop(seq).pages)
 
     # ------------------------------------------------------------------ a forward over new tokens
     def pages_needed(self, seq: int, new: int) -> int:
