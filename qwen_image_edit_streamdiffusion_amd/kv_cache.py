@@ -123,18 +123,24 @@ class PagedKVCache:
         need = [self.pages_needed(s, n) for s, n in zip(seqs, new)]
         if sum(need) > len(self._free):
             raise CacheFull(f"{sum(need)} pages wanted, {len(self._free)} of {self.num_pages} free")
-        P, slots, lens, cu = self.page_size, [], [], [0]
+        P, slots, lens, cu, table = self.page_size, [], [], [0], []
+        free = iter(reversed(self._free))  # in the order in which _take gives them
         for seq, n, m in zip(seqs, new, need):
             s = self._seqs[seq]
-            s.pages += self._take(m)
-            slots += [s.pages[i // P] * P + i % P for i in range(s.length, s.length + n)]
-            s.length += n
-            lens.append(s.length)
+            pages = s.pages + [next(free) for _ in range(m)]
+            slots += [pages[i // P] * P + i % P for i in range(s.length, s.length + n)]
+            lens.append(s.length + n)
             cu.append(cu[-1] + n)
-        width = max(1, max(len(self._seqs[s].pages) for s in seqs))
-        table = [self._seqs[s].pages + [0] * (width - len(self._seqs[s].pages)) for s in seqs]
+            table.append(pages)
+        width = max(1, max(map(len, table)))
         i32 = lambda v: torch.tensor(v, dtype=torch.int32).to(self.device)  # noqa: E731
-        return CacheStep(i32(table), i32(lens), i32(cu), torch.tensor(slots, dtype=torch.int64).to(self.device))
+        step = CacheStep(i32([t + [0] * (width - len(t)) for t in table]), i32(lens), i32(cu),
+                         torch.tensor(slots, dtype=torch.int64).to(self.device))
+        for seq, n, m in zip(seqs, new, need):  # the arrays are there: the tokens count
+            s = self._seqs[seq]
+            s.pages += self._take(m)
+            s.length += n
+        return step
 
     def take_back(self, seqs: Sequence[int], new: Sequence[int]) -> None:
         """Undo the last ``step`` of these sequences, as where its forward failed: the tokens are no longer
