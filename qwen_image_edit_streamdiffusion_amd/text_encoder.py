@@ -271,10 +271,11 @@ class QwenVLTextModel:
     def forward_packed(self, prompts: Sequence[torch.Tensor],
                        position_ids: Optional[Sequence[torch.Tensor]] = None) -> List[torch.Tensor]:
         """Several prompts in one pass: token ids [S_i] or embeddings [S_i, D] each, positions [3, S_i]
-        (default: 0..S_i-1 on all three axes) -> their last hidden states [S_i, D], as ``forward`` of each."""
+        or [S_i] (default: 0..S_i-1 on all three axes) -> their last hidden states [S_i, D], as ``forward`` of each."""
         lens = [int(p.shape[0]) if p.is_floating_point() else int(p.numel()) for p in prompts]
         if position_ids is None:
             position_ids = [torch.arange(n).view(1, n).expand(3, n) for n in lens]
+        position_ids = self._axes_positions(position_ids, lens)
         cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32).to(self.device)
         H, Hk, Dh = self.config.num_attention_heads, self.config.num_key_value_heads, self.config.head_dim
 
@@ -294,7 +295,7 @@ class QwenVLTextModel:
         if position_ids is None:
             position_ids = [torch.arange(cache.length(s), cache.length(s) + n).view(1, n).expand(3, n)
                             for s, n in zip(seqs, lens)]
-        self._check_positions(position_ids, lens)
+        position_ids = self._axes_positions(position_ids, lens)
         st = cache.step(seqs, lens)
         c = self.config
         H, Hk, Dh = c.num_attention_heads, c.num_key_value_heads, c.head_dim
@@ -312,11 +313,13 @@ class QwenVLTextModel:
             cache.take_back(seqs, lens)  # their k / v may be missing
             raise
 
-    def _check_positions(self, position_ids, lens):
+    def _axes_positions(self, position_ids, lens) -> List[torch.Tensor]:
+        """[3, n] each; one row serves all three axes."""
         if not self.layers:
             raise RuntimeError("text encoder weights not loaded")
-        if len(position_ids) != len(lens) or any(tuple(p.shape) != (3, n) for p, n in zip(position_ids, lens)):
-            raise ValueError("positions [3, tokens] for each sequence")
+        if len(position_ids) != len(lens) or any(tuple(p.shape) not in ((3, n), (1, n), (n,)) for p, n in zip(position_ids, lens)):
+            raise ValueError("positions [3, tokens], or [tokens] for all three axes, for each sequence")
+        return [p.cpu().expand(3, n) for p, n in zip(position_ids, lens)]
 
     def _rows(self, prompts, position_ids, lens, attend) -> torch.Tensor:
         """The layers over the rows of all sequences, one behind the other; ``attend(layer, qkv, q, positions, out)``
@@ -324,11 +327,10 @@ class QwenVLTextModel:
         c, w, dev = self.config, self.w, self.device
         D, H, Hk, Dh, F = c.hidden_size, c.num_attention_heads, c.num_key_value_heads, c.head_dim, c.intermediate_size
         T = sum(lens)
-        self._check_positions(position_ids, lens)
         h = torch.empty(T, D, dtype=BF16, device=dev)
         if T == 0:
             return h
-        pos = torch.cat([p.cpu() for p in position_ids], 1).to(torch.int32).to(dev)
+        pos = torch.cat(list(position_ids), 1).to(torch.int32).to(dev)
         x = torch.empty(T, D, dtype=BF16, device=dev)
         at = 0
         for p, n in zip(prompts, lens):
