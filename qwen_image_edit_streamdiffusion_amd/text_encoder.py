@@ -421,7 +421,6 @@ class QwenVLEncoder:
         from .vision import QwenVLVisionTower, VisionConfig
         self.text = QwenVLTextModel(text_config, device, packed_attention)
         self.vision = QwenVLVisionTower(vision_config or VisionConfig(), device, packed_attention)
-        self.packed_attention = packed_attention
         self.prefix_cache_size = prefix_cache_size
         self.prefix_pages = prefix_cache_pages or 16 * (prefix_cache_size + 1)
         self.prefixes: "OrderedDict[int, _Prefix]" = OrderedDict()  # cache sequence -> what it holds
@@ -435,6 +434,15 @@ class QwenVLEncoder:
         # (the realtime loop's case) re-runs only the language model
         self.vision_cache: "OrderedDict[tuple, torch.Tensor]" = OrderedDict()
         self.vision_cache_size = vision_cache_size
+
+    @property
+    def packed_attention(self) -> bool:
+        """Both models' switch; may be set at any time."""
+        return self.text.packed_attention and self.vision.packed_attention
+
+    @packed_attention.setter
+    def packed_attention(self, on: bool) -> None:
+        self.text.packed_attention = self.vision.packed_attention = bool(on)
 
     def load_state_dict(self, sd: Dict[str, torch.Tensor]) -> "QwenVLEncoder":
         self.clear_prefixes()

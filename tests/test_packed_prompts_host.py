@@ -37,3 +37,22 @@ def test_positions_of_one_row_serve_all_axes(model):
     with pytest.raises(ValueError):
         model.extend(cache, [s], [ids], [row[:4]])
     assert cache.length(s) == 0
+
+
+def test_the_encoders_switch_is_its_models():
+    """Set after the load, as on the encoder that a pipeline holds: both models and the batch follow."""
+    from qwen_image_edit_streamdiffusion_amd.text_encoder import QwenVLEncoder, TextEncoderConfig
+    from qwen_image_edit_streamdiffusion_amd.vision import VisionConfig
+    make = lambda **kw: QwenVLEncoder(  # noqa: E731
+        TextEncoderConfig(vocab_size=100, hidden_size=256, intermediate_size=512, num_hidden_layers=1, num_attention_heads=2,
+                          num_key_value_heads=1),
+        VisionConfig(depth=1, hidden_size=320, intermediate_size=200, num_heads=4, out_hidden_size=256, fullatt_block_indexes=(0,)),
+        "cpu", **kw)
+    state = lambda e: (e.packed_attention, e.text.packed_attention, e.vision.packed_attention)  # noqa: E731
+    enc = make()
+    assert state(enc) == (False, False, False)
+    enc.packed_attention = True
+    assert state(enc) == (True, True, True)
+    enc.packed_attention = False
+    assert state(enc) == (False, False, False)
+    assert state(make(packed_attention=True)) == (True, True, True)
