@@ -363,6 +363,7 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
 //     164 [197]; shared heads from 3500 or 1500: 12 over 4, 4 x 4000 151 [156]). Over a cache, for more than 2048 keys (6 x 600 over 3000: 180 [188]; 3 x 1500 over 1500: 85 [76]; heads
 //     of 64 4096), where little of a block is padding: a sixth (6 x 600 over 3000, 16 heads of 80, 18 blocks for 14:
 //     160 [106]), a third where shares even out the rest (10 of up to 758 over up to 9770: 402 [458]).
+constexpr double kMostParts = 256 << 20;
 struct SeqPlan {
   int bm, waves, ct, maxch, shares;
 };
@@ -429,6 +430,11 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, int head_dim, bo
   const double low = p.bm < kBM ? fmax(4.0, 0.6 * sqrt(tiles)) : 8;
   double ct = fmax(tiles / n, low);
   if (per <= 64 || tiles > 128) ct = fmin(ct, groups >= 256 || (per > 64 && seqs == 1) ? 64 : fmax(32.0, low));
+  // The parts go by what the table could hold, for the lengths are not known here: kMostParts bytes of them at most.
+  // Where fewer than two chunks of them fit, q alone is 64 MiB: thousands of blocks, no cut needed to fill the chip.
+  const double fit = floor(kMostParts / ((double)tokens * heads * (head_dim + 2) * 4));
+  if (fit < 2) return p;
+  ct = fmax(ct, tiles / fit);
   if (tiles > ct) {
     p.ct = (int)ceil(tiles / ceil(tiles / ct - 1e-9));  // chunks of one size
     p.maxch = (int)ceil(tiles / p.ct);
