@@ -419,8 +419,10 @@ int qie_rope_append_bf16(const void* qkv, int64_t ldx, void* q_out, int64_t ldo,
 /* Attention within each of `seqs` packed sequences: rows [cu_seqlens[b], cu_seqlens[b + 1]) of q
  * [tokens][heads][head_dim] over the same rows of k, v [tokens][kv_heads][head_dim] (query head h
  * reads kv head h / (heads / kv_heads)); causal: key j <= query i. fp32 softmax, P rounded to bf16
- * for P.V. What a query does not see does not reach it, infinities and NaN included. Rows outside
- * every sequence are left as they were. Strides in elements, multiples of 8; head_dim % 8 == 0,
+ * for P.V. What a query does not see does not reach it, infinities and NaN included. Scores are
+ * fp32: a product past its range is an infinity; a row whose visible scores are all -inf is 0, as one
+ * that sees no key. scale * score is to stay in that range too. Rows outside every sequence are left
+ * as they were. Strides in elements, multiples of 8; head_dim % 8 == 0,
  * <= 128; 0 < scale <= 65536; out: q itself or memory apart from it (in the next one as well). */
 int qie_attention_packed_bf16(const void* q, int64_t ldq, int64_t hsq, const void* k, const void* v, int64_t ldk,
                               int64_t hsk, const int* cu_seqlens, int seqs, int tokens, int heads, int kv_heads,

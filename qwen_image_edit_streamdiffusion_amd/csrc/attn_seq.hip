@@ -121,7 +121,8 @@ __global__ void __launch_bounds__(256, WGS) attn_seq_kernel(SeqArgs a) {
   f32x4_t o[ND];
 #pragma unroll
   for (int db = 0; db < ND; ++db) o[db] = f32x4_t{};
-  float m_run = kLow, l_run = 0.f;
+  float m_run = a.low, l_run = 0.f;
+  float above = kRescale, mscale = a.c;  // seq_far
 
   __builtin_amdgcn_s_waitcnt(0);  // q and two tiles: from here on the counter is the tiles'
   asm volatile("s_barrier" ::: "memory");
@@ -176,15 +177,18 @@ __global__ void __launch_bounds__(256, WGS) attn_seq_kernel(SeqArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[kb][i]);
     mx = quad_max(mx);
-    if (__any((mx - m_run) * a.c > kRescale)) {
+    if (__any((mx - m_run) * a.c > above)) {
       const float m_new = fmaxf(m_run, mx);
       const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * a.c);
       m_run = m_new;
       l_run *= alpha;
 #pragma unroll
       for (int db = 0; db < ND; ++db) o[db] *= alpha;
+      if (__builtin_expect(seq_far(a, m_run, above, mscale), 0))
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] -= m_run;
     }
-    const float mc = m_run * a.c;
+    const float mc = m_run * mscale;
     bf16x8_t pf;
     float p[8];
 #pragma unroll
@@ -303,7 +307,7 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
   const int d = 2 * lane;
   const float* po = a.ws + row * a.maxch * a.Dh + (d < a.Dh ? d : 0);
   constexpr int kAhead = 8;
-  f32x2_t ml = f32x2_t{kLow, 0.f}, v[kAhead], w[kAhead];
+  f32x2_t ml = f32x2_t{a.low, 0.f}, v[kAhead], w[kAhead];
   if (lane < nch) ml = *(const f32x2_t*)(pml + 2 * lane);
   auto fetch = [&](f32x2_t* to, int from) {  // past the last chunk: the last once more, its weight is 0 then
 #pragma unroll
@@ -316,7 +320,7 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
   float l = 0.f, o0 = 0.f, o1 = 0.f;
   for (int c0 = 0; c0 < nch; c0 += 64) {  // a lane weighs a chunk, then all lanes add 64 chunks' rows
     if (c0 > 0) {
-      ml = f32x2_t{kLow, 0.f};
+      ml = f32x2_t{a.low, 0.f};
       if (c0 + lane < nch) ml = *(const f32x2_t*)(pml + 2 * (c0 + lane));
     }
     const float wt = c0 + lane < nch ? __builtin_amdgcn_exp2f((ml[0] - mx) * a.c) : 0.f;
@@ -472,6 +476,11 @@ int launch_seq(SeqArgs& a, const SeqPlan& p, bool paged, hipStream_t s) {
   return qie_last_error();
 }
 
+void set_scale(SeqArgs& a, float scale) {
+  a.c = scale * 1.4426950408889634f;
+  a.low = -3e38f / fmaxf(a.c, 1.f);
+}
+
 bool seq_common_ok(const void* q, int64_t ldq, int64_t hsq, const void* k, const void* v, int64_t ldk, int64_t hsk,
                    int seqs, int tokens, int heads, int kv_heads, int head_dim, float scale, const void* out,
                    int64_t ldo, int64_t hso) {
@@ -499,7 +508,7 @@ extern "C" int qie_attention_packed_bf16(const void* q, int64_t ldq, int64_t hsq
   a.cu = cu_seqlens;
   a.B = seqs; a.T = tokens; a.H = heads; a.Hk = kv_heads; a.G = heads / kv_heads; a.Dh = head_dim;
   a.causal = causal != 0;
-  a.c = scale * 1.4426950408889634f;
+  set_scale(a, scale);
   return launch_seq(a, seq_plan(tokens, seqs, heads, kv_heads, head_dim, causal != 0, 0), false, (hipStream_t)stream);
 }
 
@@ -538,7 +547,7 @@ extern "C" int qie_attention_paged_bf16(const void* q, int64_t ldq, int64_t hsq,
   a.cu = cu_seqlens;
   a.B = seqs; a.T = tokens; a.H = heads; a.Hk = kv_heads; a.G = heads / kv_heads; a.Dh = head_dim;
   a.causal = 1;
-  a.c = scale * 1.4426950408889634f;
+  set_scale(a, scale);
   a.table = page_table; a.ldt = ld_table; a.ps = page_stride;
   a.kv_lens = kv_lens;
   a.width = table_width; a.pages = num_pages; a.pshift = __builtin_ctz(page_size);

@@ -107,9 +107,12 @@ __global__ void __launch_bounds__(64 * NW) attn_seq_few_kernel(SeqArgs a) {
   const int lim0 = uni(lim[0]);
   f32x4_t o[MT][ND];
   float m_run[MT], l_run[MT];
+  float above[MT], mscale[MT];  // seq_far
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    m_run[mt] = kLow;
+    m_run[mt] = a.low;
+    above[mt] = kRescale;
+    mscale[mt] = a.c;
     l_run[mt] = 0.f;
 #pragma unroll
     for (int db = 0; db < ND; ++db) o[mt][db] = f32x4_t{};
@@ -154,15 +157,18 @@ __global__ void __launch_bounds__(64 * NW) attn_seq_few_kernel(SeqArgs a) {
 #pragma unroll
       for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[mt][i >> 2][i & 3]);
       mx = quad_max(mx);
-      if (__any((mx - m_run[mt]) * a.c > kRescale)) {
+      if (__any((mx - m_run[mt]) * a.c > above[mt])) {
         const float m_new = fmaxf(m_run[mt], mx);
         const float alpha = __builtin_amdgcn_exp2f((m_run[mt] - m_new) * a.c);
         m_run[mt] = m_new;
         l_run[mt] *= alpha;
 #pragma unroll
         for (int db = 0; db < ND; ++db) o[mt][db] *= alpha;
+        if (__builtin_expect(seq_far(a, m_run[mt], above[mt], mscale[mt]), 0))
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s[mt][i >> 2][i & 3] -= m_run[mt];
       }
-      const float mc = m_run[mt] * a.c;
+      const float mc = m_run[mt] * mscale[mt];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][i >> 2][i & 3], a.c, -mc));
@@ -244,7 +250,7 @@ __global__ void __launch_bounds__(64 * NW) attn_seq_few_kernel(SeqArgs a) {
       mw[w] = *(const f32x2_t QIE_LDS*)&ml[w][row][0];
       v[w] = *(const f32x4_t QIE_LDS*)(smem + w * 2 * kFTile + row * 512 + ((ch ^ (row & 15)) << 4));
     }
-    float M = kLow;
+    float M = a.low;
 #pragma unroll
     for (int w = 0; w < NW; ++w) M = fmaxf(M, mw[w][0]);
     float L = 0.f;

@@ -253,7 +253,8 @@ __global__ void __launch_bounds__(512) attn_seq_pp_kernel(SeqArgs args) {
   bf16x8_t qf[KS];
   f32x16_t s[2], o[ND];
   bf16x8_t pf[4];
-  float m_run = kLow, l_run = 0.f;
+  float m_run = a.low, l_run = 0.f;
+  float above = kRescale, mscale = a.c;  // seq_far
 #pragma unroll
   for (int db = 0; db < ND; ++db) o[db] = f32x16_t{};
 
@@ -384,15 +385,18 @@ __global__ void __launch_bounds__(512) attn_seq_pp_kernel(SeqArgs args) {
       const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
       mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
     }
-    if (__any((mx - m_run) * a.c > kRescale)) {
+    if (__any((mx - m_run) * a.c > above)) {
       const float m_new = fmaxf(m_run, mx);
       const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * a.c);
       m_run = m_new;
       l_run *= alpha;
 #pragma unroll
       for (int db = 0; db < ND; ++db) o[db] *= alpha;
+      if (__builtin_expect(seq_far(a, m_run, above, mscale), 0))
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s[i >> 4][i & 15] -= m_run;
     }
-    const float mc = m_run * a.c;
+    const float mc = m_run * mscale;
     float ps0 = 0.f, ps1 = 0.f;
 #pragma unroll
     for (int cb = 0; cb < 2; ++cb)
@@ -586,7 +590,7 @@ __global__ void __launch_bounds__(256) attn_seq_join_shares_kernel(SeqArgs a) {
   float m[kJoinRows], L[kJoinRows], o0[kJoinRows], o1[kJoinRows];
 #pragma unroll
   for (int j = 0; j < kJoinRows; ++j) {
-    m[j] = kLow;
+    m[j] = a.low;
     L[j] = o0[j] = o1[j] = 0.f;
   }
   for (int i0 = s - 1; i0 < ns && cut(i0) < l.c1; i0 += 64) {

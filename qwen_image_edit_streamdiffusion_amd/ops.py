@@ -736,7 +736,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     """Attention within packed sequences: rows [cu_seqlens[b], cu_seqlens[b + 1]) (device int32
     [seqs + 1], ascending) of q [T, H, Dh] over the same rows of k, v [T, Hk, Dh], H a multiple of Hk;
     ``causal``: key j <= query i. Views of one projection's columns are fine. A query's result holds
-    nothing of the keys it does not see. Rows outside every sequence are left as they were (``out``
+    nothing of the keys it does not see. Scores, and scores times scale, are 32-bit: a row whose visible scores are
+    all -inf is 0, as one that sees none. Rows outside every sequence are left as they were (``out``
     given: q itself or memory apart from q, k and v) or undefined."""
     return (_seq_calls or _seq()).attention_packed(q, k, v, cu_seqlens, out, causal, scale)
 
