@@ -418,13 +418,13 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, int head_dim, bo
   const double half = per > 16 ? 0.5 * seqs * kv_heads : 0;  // sequences end inside a block
   const double groups = p.bm == 16 ? g16 + half : p.bm == 32 ? g32 + half : p.bm == kBM ? g64 / 3 : g256 + half;
   // Many rows over more than 4096 keys, half of them kept at least: equal shares of the call's work (1500, 1100 and
-  // 700 new tokens over 24000, 11000 and 7000: 737 [836 in chunks]; 8 x 300 over 3000 and 9000: 251 [302]; of one
-  // length, 8 x 200 over 5000, whole blocks again, 146 [141]). From 512 groups on whole blocks even out (4 x 2000 over
-  // 2000 .. 9000: 439 [516 in shares]), and a single sequence's do where they fill their rounds (3500 new tokens, 383
-  // groups, over 24000: 1047 in shares [1183]; 2340, 256 groups: 735 whole [791]). The sum of all blocks' keys has to fit
-  // the shares' 32 bits.
+  // 700 new tokens over 24000, 11000 and 7000: 715 [814 in chunks of 64 tiles]; 8 x 300 over 3000 and 9000: 242 [270];
+  // of one length, 8 x 200 over 5000, the kernel goes back to whole blocks: 147 [138 without the line]). One sequence
+  // too, also where its blocks fill their rounds (383 of them, 3500 new tokens over 24000: 1030 [1205 whole]; 256 of
+  // them, 2340 tokens: 710 [700 whole, 793 in chunks]). From 512 blocks on whole ones even out (4 x 2000 over 2000 ..
+  // 9000: 515 [615 in shares]). The sum of all blocks' keys has to fit the shares' 32 bits.
   if (p.bm == kPPRows && tiles > 64 && keys * seqs >= 2.0 * tokens && (g256 + seqs) * (keys + tokens + 1024) < 3e10 &&
-      (seqs > 1 ? groups < 512 : g256 < 0.88 * 256 * rounds)) {
+      groups < 512) {
     p.shares = kv_heads <= 256 ? 256 / kv_heads : 1;
     return p;
   }

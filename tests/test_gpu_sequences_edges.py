@@ -142,3 +142,14 @@ def test_scores_past_32_bits():
     got = ops.attention_packed(d(q), d(k), d(v), torch.tensor([0, 4], dtype=torch.int32, device=DEV)).cpu()
     assert not got[:2].any() and torch.equal(got[2], v[2]) and torch.equal(got[3], v[2])
     assert math.isinf(float(q[0, 0, 0] * k[0, 0, 0]))
+
+
+def test_one_sequence_that_fills_the_chip_over_a_long_cache():
+    """As many 256-row blocks as the chip has places, in equal shares."""
+    ops = _ops()
+    new, kv, H, Dh, P = [1900], [4200], 32, 64, 64
+    q, ks, vs, kp, vp, table = _paged(_gen(5), new, kv, H, H, Dh, P)
+    want, tol = paged_ref(q, ks, vs, new, kv)
+    got = ops.attention_paged(q.to(DEV), kp, vp, table.to(DEV), torch.tensor(kv, dtype=torch.int32, device=DEV),
+                              cu_seqlens=_cu(new).to(DEV))
+    _check(got, want, tol)

@@ -38,3 +38,9 @@ def test_few_rows_over_a_long_table_are_still_cut(bytes_of):
     """A bound that left no cut would put a single token's 32768 keys on four work-groups."""
     assert bytes_of(1, 1, 28, 4, 128, 512, 64) >= 28 * 8 * 130 * 4
     assert bytes_of(128, 32, 28, 4, 128, 512, 64) > 0 and bytes_of(1 << 20, 1, 1, 1, 128, 1 << 18, 64) >= 0
+
+
+@pytest.mark.parametrize("new,table", [(2200, 24000), (2340, 24000), (2340, 1 << 17), (4500, 24000), (4600, 12000)])
+def test_one_sequence_whose_blocks_fill_the_chip_is_not_cut_in_chunks(bytes_of, new, table):
+    """It takes equal shares as any other: two blocks of 256 rows of parts for each of 256 work-groups."""
+    assert bytes_of(new, 1, 28, 4, 128, table // 64, 64) == 256 * 2 * 256 * 130 * 4
