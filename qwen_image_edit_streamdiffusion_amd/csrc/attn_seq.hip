@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(256, WGS) attn_seq_kernel(SeqArgs a) {
       return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
     };
     // V is read ahead of the exponentials; where four work-groups of 128-wide heads share a CU, a masked tile has
-    // no registers to keep it in (184 bytes spilled, 333 us in place of 196 for 64 prompts of 400)
+    // no registers to keep it in (184 bytes spilled, 318 us in place of 174 for 64 prompts of 400)
     constexpr bool KEEP = !MASKED || NK < 4 || WGS < 4;
     bf16x8_t vv[ND];
     if constexpr (KEEP) {
@@ -346,27 +346,41 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
 
 // Which kernel, and how the keys are cut, by what the host knows: tokens, sequences, heads and the
 // longest cache that a table can hold (packed sequences: their mean length). Rows are those of one kv
-// head, tokens * G; a group is a (row block, kv head). Times in us, bf16, head_dim 128, 28 heads over 4
-// unless said, the other side in brackets.
-//   few rows (attn_seq_few), 16-row blocks: up to 256 groups with eight waves each (one prompt of 100 tokens 7.3
-//     [8.0 in 64-row blocks]), up to 512 with four, two a CU (one prompt of 200: 8.4 [10.9 with eight, 9.3 in 64-row
-//     blocks]), and more than that over up to 1500 keys (80 tokens of 24 heads over 24, caches of 20, 300 and 1000: 17,
-//     49 and 170 [27, 60 and 170 with eight]; over 8000 eight again: 1277 [1287 with four]). 32-row blocks over more
-//     than 256 keys where 16-row ones would be more than 256 (200 new tokens over 1000: 14.4 [17.0]; 10 x 20 over 300,
-//     16 heads of 80, 8.6 [10.1]), or read a long cache again and again (4 new tokens over 20000 keys of 16 sequences:
-//     135 [189]).
-//   64-row blocks (attn_seq): shorter packed sequences (16 prompts of 400: 46 [53 in 256-row blocks]; from 200 groups
-//     on very short ones, 16 x 30, 16 heads of 80: 5.6 [7.0 in 16-row blocks]), a short
-//     cache's many rows (16 x 100 new tokens over 300: 21 [23]), and 33 .. 64 rows of a sequence over a long one (16 x
-//     8 new tokens over 20000: 138 [201 in 32-row blocks]).
-//   256-row blocks (attn_seq_pp) for packed sequences where there are 200 of them, their rounds are full enough, and the
-//     mean length is 700 (10 x 1000: 122 [126 in 64-row blocks]; 5 x 2000: 173 [191]; 1500 where causal heads share
-//     nothing and a block spans 256 tokens: 10 x 1000, 24 heads over 24, 118 [104]). Narrow heads cost them as much as
-//     wide ones: from 1800 causal or 1000 full rows at 65 .. 96 (7 x 1500, 16 heads of 80: 100 [85]; 4 x 3000: 145 [153];
-//     full 7 x 1500: 122 [135]), from 5000 or 3500 at 64 (8 heads, 4 x 3000: 90 [75], 4 x 8000: 374 [402]; full 4 x 4000:
-//     164 [197]; shared heads from 3500 or 1500: 12 over 4, 4 x 4000 151 [156]). Over a cache, for more than 2048 keys (6 x 600 over 3000: 180 [188]; 3 x 1500 over 1500: 85 [76]; heads
+// head, tokens * G; a group is a (row block, kv head). Times in us (device, median), bf16, head_dim 128, 28 heads
+// over 4 unless said, the other side in brackets.
+//   few rows (attn_seq_few), 16-row blocks: up to 256 groups with eight waves each (one prompt of 100 tokens 5.8
+//     [6.9 in 64-row blocks]), up to 512 with four, two a CU (one prompt of 200: 7.7 [9.9 with eight, 8.2 in 64-row
+//     blocks]; of 280: 8.8 [9.3]; past it, one of 300: 10.0 in 64-row blocks [11.2]), and more than that over up to 1500
+//     keys (80 tokens of 24 heads over 24, caches of 20, 300 and 1000: 16, 49 and 171 [26, 59 and 171 with eight]; over
+//     8000, eight and four are level at 1300). 32-row blocks over more than 256 keys where 16-row ones would be more than
+//     256 (200 new tokens over 1000: 13.8 [16.4 in 16-row, 25.9 in 64-row blocks]; 10 x 20 over 300, 16 heads of 80, 7.7
+//     [9.6]), or where a cache is read again for each 16 rows and that takes longer than the second half of a block: for
+//     17 .. 32 rows a sequence from groups * keys = 6e4 on (3 new tokens over 6000 keys of one sequence 10.8 in 16-row
+//     blocks [12.5], over 20000 17.7 in 32-row ones [21.5]; 4 over 20000 of 16 sequences 138 [194]), for more rows from 4e5
+//     (8 over 20000 of one sequence: 21.0 in 16-row blocks [22.8]), and up to 1.5e6 against larger blocks (70 over 20000:
+//     68 [94 in 64-row ones]; 100: 79 in 256-row ones [128]).
+//   64-row blocks (attn_seq): shorter packed sequences (16 prompts of 400: 43 [53 in 256-row blocks]; from 200 groups
+//     on very short ones, 16 x 30, 16 heads of 80: 4.7 [6.2 in 16-row blocks]), a short
+//     cache's many rows (16 x 100 new tokens over 300: 19.5 [22.5 in 256-row blocks]), and 33 .. 64 rows of a sequence
+//     over a long one where 32-row ones are more than 3e5 groups * keys (3 x 8 new tokens over 20000: 31 [59]; 16 x 8 135
+//     [203]).
+//   256-row blocks (attn_seq_pp) for packed sequences where there are 200 of them (2 x 1150, 252: 37 [39 in 64-row
+//     blocks]; 4 x 650, 182: 29 in 64-row ones [31]), their rounds of 256 are two thirds full (2 x 1600, 350: 49 [55]; 2 x
+//     1371, 300: level at 48), and the mean length is at least
+//       head_dim      causal, shared heads          causal, not shared             full
+//       97 .. 128     1100 (8 x 1100 103 [103],     2300 (4 x 2200 158 [160],      900 (4 x 900 65 [69],
+//                     8 x 1300 129 [135],           24 heads, 4 x 1800 152 [123])  4 x 700 52 [45])
+//                     8 x 900 82 [76])
+//       65 .. 96      1800 (16 over 2, 8 x 1800     2300 (16, 4 x 2500 113 [117],  900 (16, 8 x 900 61 [64],
+//                     113 [119], 8 x 1400 79 [78])  4 x 2000 91 [81])              8 x 800 54 [50])
+//       .. 64         3500 (12 over 4, 8 x 3500     6500 (8, 4 x 7000 289 [297],   1500 or 2700 (12 over 4, 6 x 1500 69 [70],
+//                     level at 235, 4 x 4500        5 x 6000 307 [281])            6 x 1200 57 [51]; 8, 5 x 3000 123 [146],
+//                     175 [187])                                                   8 x 2500 156 [155])
+//     (narrow heads cost them as much as wide ones, and where heads share nothing a causal block spans 256 tokens). Over a
+//     cache, for more than 2048 keys (6 x 600 over 3000: 174 [185]; 3 x 1500 over 1500: 85 [75]; heads
 //     of 64 4096), where little of a block is padding: a sixth (6 x 600 over 3000, 16 heads of 80, 18 blocks for 14:
-//     160 [106]), a third where shares even out the rest (10 of up to 758 over up to 9770: 402 [458]).
+//     157 [104]), a third where shares even out the rest (10 of up to 758 over up to 9770: 423 [548]; 6 x 600 over 5000,
+//     16 heads of 80, 176 [172]; past it, 20 x 160 over 5000, 16 heads: 265 [239]).
 constexpr double kMostParts = 256 << 20;
 struct SeqPlan {
   int bm, waves, ct, maxch, shares;
@@ -381,9 +395,10 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, int head_dim, bo
   const double r16 = (double)kv_heads * seqs * ceil(per / 16), r32 = (double)kv_heads * seqs * ceil(per / 32);  // as rounded
   const int few16 = r16 <= 256 ? 8 : 4;
   // from what length on 256-row blocks pay, and how full their rounds of 256 are
-  const double longest = head_dim > 96  ? (causal && heads == kv_heads ? 1500 : 700)
-                         : head_dim > 64 ? (causal ? 1800 : 1000)
-                         : heads == kv_heads ? (causal ? 5000 : 3500) : (causal ? 3500 : 1500);
+  const bool shared = heads > kv_heads;
+  const double longest = head_dim > 64 ? (!causal ? 900 : !shared ? 2300 : head_dim > 96 ? 1100 : 1800)
+                         : shared      ? (causal ? 3500 : 1500)
+                                       : (causal ? 6500 : 2700);
   const double rounds = ceil(g256 / 256), pad = ceil(per / kPPRows) * kPPRows / per;
   SeqPlan p{kBM, few16, 0, 1, 0};
   if (!paged) {
@@ -400,19 +415,22 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, int head_dim, bo
   } else if (per > 32 && per <= 64 && g32 * keys > 3e5) {
     p.bm = kBM;
   } else if (per <= 32 || (g32 <= 512 && g32 * keys <= 1.5e6)) {
-    p.bm = r16 <= 256 && g16 * keys <= 4e5 ? 16 : 32;
+    p.bm = r16 <= 256 && g16 * keys <= (per <= 32 ? 6e4 : 4e5) ? 16 : 32;
     if (p.bm == 32) p.waves = 8;
   } else {
     p.bm = keys > (head_dim > 64 ? 2048 : 4096) && pad <= (keys > 4096 ? 1.5 : 1.2) ? kPPRows : kBM;
   }
   // Cuts: groups that do not fill the chip share a row's keys, in chunks whose fp32 parts a second kernel
-  // joins: as many as fit 256 CUs at once (1000 new tokens over 5000 keys, two of 40 tiles: 99 [uncut 134, three
-  // chunks 120]; three 64-row work-groups fit a CU), of 8 tiles at least. Up to 1024 keys, none (one token over
-  // 800: 8.5 in one launch [9.9 in two]). Few rows: 0.6 sqrt(tiles) tiles and 4 at least, where a chunk's time and
-  // the join's meet (one token over 2000, 8000 and 32768 keys: 9.8, 11.9 and 20.3 [10.9, 13.2 and 21.5 with 8 and
+  // joins: as many as fit 256 CUs at once (1000 new tokens over 4000 keys, two chunks: 86 [uncut 111, three
+  // chunks 106]; three 64-row work-groups fit a CU), of 8 tiles at least; two also where they are up to 290 (1250 over
+  // 4000, 278: 108 [111 uncut]; 1400, 308: 111 uncut [119]). Up to 1024 keys, none (one token over
+  // 800: 7.8 in one launch [8.7 in two]). Few rows: 0.6 sqrt(tiles) tiles and 4 at least, where a chunk's time and
+  // the join's meet (one token over 2000, 8000 and 32768 keys: 9.0, 11.2 and 19.4 [10.4, 12.6 and 20.9 with 8 and
   // 1.4 sqrt(tiles)]). Long tables are cut all the same, so that a long sequence among short ones is shared (48
-  // tokens over 900 .. 32768 keys: 163 [318 uncut]): into 32 tiles (4 new tokens over 20000 keys of 16 sequences: 135
-  // [142 with 64]), 64 where there is one sequence or the groups fill the chip without a cut.
+  // tokens over 900 .. 32768 keys: 167 [326 uncut]): into 32 tiles (4 new tokens over 20000 keys of 16 sequences: 138
+  // [146 with 64]), 64 where there is one sequence or the groups fill the chip without a cut. The cuts go by the table:
+  // 16 tokens over 70 .. 600 keys take 7.1 in a table of that width, 9.1 in one of 2560 .. 32768 keys, 18.6 in one of
+  // 131072.
   const double tiles = (double)((table_keys + kKB - 1) / kKB);
   if (tiles <= 16 || (p.bm == kBM && tiles <= 32)) return p;
   const double half = per > 16 ? 0.5 * seqs * kv_heads : 0;  // sequences end inside a block
@@ -449,7 +467,7 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, int head_dim, bo
 template <bool PAGED>
 int launch(const SeqArgs& a, unsigned grid, hipStream_t s) {
   // 128-wide heads fit four work-groups a CU with a register spilled (where V holds infinities): taken where more
-  // than three a CU are there (64 prompts of 400: 196 us [211 with three]; six prompts 16.7 [16.5])
+  // than three a CU are there (64 prompts of 400: 174 us [184 with three]; six of 70 .. 420 18.5 [18.2 with three])
   if (a.Dh <= 64) attn_seq_kernel<PAGED, 2, 4><<<grid, 256, 0, s>>>(a);
   else if (a.Dh <= 96) attn_seq_kernel<PAGED, 3, 4><<<grid, 256, 0, s>>>(a);
   else if (grid > 3 * 256) attn_seq_kernel<PAGED, 4, 4><<<grid, 256, 0, s>>>(a);
