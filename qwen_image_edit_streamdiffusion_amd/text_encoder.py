@@ -422,7 +422,7 @@ class QwenVLEncoder:
         self.text = QwenVLTextModel(text_config, device, packed_attention)
         self.vision = QwenVLVisionTower(vision_config or VisionConfig(), device, packed_attention)
         self.prefix_cache_size = prefix_cache_size
-        self.prefix_pages = prefix_cache_pages or 16 * (prefix_cache_size + 1)
+        self._prefix_pages = prefix_cache_pages
         self.prefixes: "OrderedDict[int, _Prefix]" = OrderedDict()  # cache sequence -> what it holds
         self.kv: Optional[PagedKVCache] = None
         if self.vision.config.out_hidden_size != self.text.config.hidden_size:
@@ -434,6 +434,11 @@ class QwenVLEncoder:
         # (the realtime loop's case) re-runs only the language model
         self.vision_cache: "OrderedDict[tuple, torch.Tensor]" = OrderedDict()
         self.vision_cache_size = vision_cache_size
+
+    @property
+    def prefix_pages(self) -> int:
+        """Pages of the kept prompts' cache, which the first of them makes."""
+        return self._prefix_pages or 16 * (self.prefix_cache_size + 1)
 
     @property
     def packed_attention(self) -> bool:

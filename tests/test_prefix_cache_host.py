@@ -181,3 +181,13 @@ def test_a_call_that_fails_at_its_end_holds_no_pages(encoder):
     assert enc.kv.free_pages == free and len(enc.prefixes) == 1
     kept.hidden = hidden
     assert _ask(enc, b) in ([100], [99], [98]) and _ask(enc, a) == []
+
+
+def test_the_size_may_be_set_after_the_load(encoder):
+    """On the encoder that a pipeline holds: pages for that many prompts, as if it had been made so."""
+    enc = encoder(0)
+    enc.prefix_cache_size = 3
+    assert enc.prefix_pages == 16 * 4
+    a, b = _ids(900, 50), _ids(800, 51)
+    assert [_ask(enc, x) for x in (a, b, a, b)] == [[900], [800], [], []]
+    assert encoder(3, pages=5).prefix_pages == 5
