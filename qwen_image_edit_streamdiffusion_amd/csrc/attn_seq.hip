@@ -16,9 +16,10 @@
 //   rescale only when a max grows by more than 2^8), P rounded to bf16 for the second product, as the
 //   matrix instruction takes it (at most 2^-8 of the mean |v| that the row sees)
 //   O^T += V^T P^T (V^T by ds_read_b64_tr_b16; the S^T registers are the P^T operand)
-// Rows past a tile's last key come from the buffer's range check as zeros. Measured: 64 windows of 16 .. 64
-// rows, 16 heads of 80, 10.2 us (2.5 TB/s); six causal prompts of 70 .. 420, 28 heads over 4, 14.9 us, whose
-// longest block walks 14 tiles one behind the other; 16 prompts of 400 46 us, 64 174 (420 TFLOP/s). Tried and
+// Rows past a tile's last key come from the buffer's range check as zeros. Measured (device, median): 64 windows
+// of 16 .. 64 rows, 16 heads of 80, 9.3 us (2.7 TB/s); six causal prompts of 70 .. 420, 28 heads over 4, 15.0 us, whose
+// longest block walks 14 tiles one behind the other; one of 300 10.0; 784 rows of 16 heads of 80, all of which see
+// each other, 15.9; 16 prompts of 400 44 us, 64 175 (420 TFLOP/s). Tried and
 // slower or equal: 64-key tiles, three stages with one barrier a tile, 32 rows a wave, two groups of waves a
 // block that share its keys, the next tile's scores beside this one's softmax.
 #include <cmath>
@@ -368,9 +369,9 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
 //     blocks]; 4 x 650, 182: 29 in 64-row ones [31]), their rounds of 256 are two thirds full (2 x 1600, 350: 49 [55]; 2 x
 //     1371, 300: level at 48), and the mean length is at least
 //       head_dim      causal, shared heads          causal, not shared             full
-//       97 .. 128     1100 (8 x 1100 103 [103],     2300 (4 x 2200 158 [160],      900 (4 x 900 65 [69],
-//                     8 x 1300 129 [135],           24 heads, 4 x 1800 152 [123])  4 x 700 52 [45])
-//                     8 x 900 82 [76])
+//       97 .. 128     1000 (10 x 1000 107 [109],    2300 (24, 4 x 2500 189 [204],  900 (4 x 900 65 [69],
+//                     8 x 1300 129 [135],           4 x 1800 152 [123])            4 x 700 52 [45])
+//                     8 x 900 80 [76])
 //       65 .. 96      1800 (16 over 2, 8 x 1800     2300 (16, 4 x 2500 113 [117],  900 (16, 8 x 900 61 [64],
 //                     113 [119], 8 x 1400 79 [78])  4 x 2000 91 [81])              8 x 800 54 [50])
 //       .. 64         3500 (12 over 4, 8 x 3500     6500 (8, 4 x 7000 289 [297],   1500 or 2700 (12 over 4, 6 x 1500 69 [70],
@@ -396,7 +397,7 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, int head_dim, bo
   const int few16 = r16 <= 256 ? 8 : 4;
   // from what length on 256-row blocks pay, and how full their rounds of 256 are
   const bool shared = heads > kv_heads;
-  const double longest = head_dim > 64 ? (!causal ? 900 : !shared ? 2300 : head_dim > 96 ? 1100 : 1800)
+  const double longest = head_dim > 64 ? (!causal ? 900 : !shared ? 2300 : head_dim > 96 ? 1000 : 1800)
                          : shared      ? (causal ? 3500 : 1500)
                                        : (causal ? 6500 : 2700);
   const double rounds = ceil(g256 / 256), pad = ceil(per / kPPRows) * kPPRows / per;

@@ -6,9 +6,9 @@
 // are made, V as soon as its product is, so a wave always has 8 KiB on the way and a work-group
 // 8 NW .. 16 NW KiB. At the end the waves' (max, sum, O) meet in LDS.
 //
-// Products as in attn_seq.hip (S^T = K Q^T and O^T += V^T P^T on mfma 16x16x32). Measured, 28 heads over 4:
-// 48 single tokens over 900 .. 32768 keys 281 us, 5.7 TB/s, and 5 for the join; 16 over 70 .. 600 7.9 us, 41 new
-// tokens over 309 6.6 (latency: launch, length and table, two or three rounds of tiles, merge).
+// Products as in attn_seq.hip (S^T = K Q^T and O^T += V^T P^T on mfma 16x16x32). Measured (device,
+// median), 28 heads over 4: 48 single tokens over 900 .. 32768 keys 284 us, 5.6 TB/s, and 5.4 for the join; 16 over 70
+// .. 600 7.6 us, 41 new tokens over 309 6.9 (latency: launch, length and table, two or three rounds of tiles, merge).
 #include "attn_seq.h"
 
 namespace {

@@ -2,16 +2,18 @@
 // heads of one kv head) of one sequence, 32 rows a wave, 64-key tiles. The products are those of
 // attn_seq.hip on mfma 32x32x16 (S^T = K Q^T, O^T += V^T P^T; a lane holds 32 keys of one row).
 //
-// Bound by the matrix pipe and, beside it, by the softmax's vector issue. Waves 0-3 and 4-7 put one
-// wave of each group on every SIMD, one phase apart: while one is in its matrix phase (S of tile t,
-// then O += V P of tile t - 1, operands read from LDS five products ahead) the other is in its
+// Waves 0-3 and 4-7 put one wave of each group on every SIMD, one phase apart: while one is in its matrix phase
+// (S of tile t, then O += V P of tile t - 1, operands read from LDS six products ahead) the other is in its
 // softmax phase. K and V live in 4-slot LDS rings; softmax phase t issues the LDS-DMA of K(t + 3) and
 // V(t + 2) and ends when what it issued a phase earlier has landed, so every tile is there two
 // phases before its first read and one barrier ends each phase. The products are asm volatile:
 // their order and the LDS reads between them stay as written; register fences pin the softmax
-// inside its phase. Measured, 28 heads of 128 over 4: four causal sequences of up to 8192 690 us (1095 TFLOP/s),
-// 32768 causal rows 1173 TFLOP/s, new tokens over 24000 cached keys 1060 .. 1085; the matrix pipe is busy 55% of the
-// cycles at the 1.9 GHz that the power limit leaves, no LDS bank conflicts.
+// inside its phase. Measured (device, median), 28 heads of 128 over 4: four causal sequences of up to 8192 690 .. 745 us
+// on one card and another (1095 .. 1015 TFLOP/s), 32768 causal rows 6.4 .. 6.7 ms (1200 .. 1150), chunks of 300 .. 1500
+// tokens over 5000 .. 24000 cached keys 505 .. 520 and 20 for the join. A tile of 128-wide heads takes a CU 3450 cycles
+// (paged: 4110): the matrix pipe of a SIMD is busy for 2048 of them, the other wave's 250 vector instructions take
+// about as many, no LDS bank conflicts. So neither unit is the bound; the phases take 1.7 times the longer of the two
+// (paged: 2), and what they wait for in between has not been separated.
 #include <type_traits>
 
 #include "attn_seq.h"
@@ -63,7 +65,7 @@ __device__ __forceinline__ LineSeq line_seq(const SeqArgs& a, int b) {
   return s;
 }
 // The line's length and how it is cut: ns equal shares; or, where no block is much longer than a share would
-// be, whole blocks (16 x 100 new tokens over 5000 keys: 150 us, 158 in shares)
+// be, whole blocks (8 x 200 new tokens over 5000 keys: 151 us, 157 in shares; 16 x 100: level at 165)
 struct Cuts {
   int total, ns;
   bool whole;

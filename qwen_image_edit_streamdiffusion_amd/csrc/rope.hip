@@ -10,9 +10,9 @@
 //
 // Bound by HBM: every head is read and written once, the angles of a token are shared by all its
 // heads. A work-group computes the cos / sin of its tokens once into LDS, then its threads walk the
-// (token, head) items, V pairs each as 16-byte accesses. Measured: 16816 rows of 48 heads of 128 77.4 us,
-// 5.34 TB/s; the append of 4099 rows of 28 + 2 x 4 heads 16.4 us, 4.6 TB/s; up to some hundred rows the
-// launch (16 rows 3.3 us, 300 rows of 32 heads 3.3, 784 of 32 80-wide heads 4.1).
+// (token, head) items, V pairs each as 16-byte accesses. Measured (device, median): 16816 rows of 48 heads of
+// 128 77 us into other memory, 5.4 TB/s, 61 in place, 6.7; the append of 4099 rows of 28 + 2 x 4 heads 14.1 us, 5.4 TB/s;
+// up to some hundred rows the launch (16 rows 3.5 us, 300 rows of 32 heads 3.4, 784 of 32 80-wide heads 4.2).
 #include <algorithm>
 
 #include "qie_common.h"
@@ -155,9 +155,9 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(RopeArgs a) {
 }
 
 // Tokens of a work-group: with fewer than 2048 rows one, so that the rows spread over the chip (300 rows of 32
-// heads: 3.0 us, 3.9 with four); else as many as give its threads two items each, for the cos and sin of a
-// token are made by the same threads (16384 rows of 8 heads: 12.5 us with four, 17.7 with one; 4096 of 32: 12.1 with
-// two, 12.9 with one; 16816 of 48: 75.5 with one, 82.8 with four).
+// heads: 3.5 us, 4.3 with four); else as many as give its threads two items each, for the cos and sin of a
+// token are made by the same threads (in place, 16384 rows of 8 heads: 11.0 us with four, 16.0 with one; 4096 of 32: 9.3
+// with two, 10.3 with one; 16816 of 48: 61.3 with one, 63.4 with four).
 int rope_tokens(const RopeArgs& a, int V) {
   if (a.T < 2048) return 1;
   return (int)std::min<int64_t>(kRopeTB, std::max<int64_t>(1, 2 * 256 / ((int64_t)a.nh * (a.pairs / V))));
@@ -166,7 +166,7 @@ int rope_tokens(const RopeArgs& a, int V) {
 template <bool APPEND>
 int launch_rope(RopeArgs& a, bool inter, hipStream_t s) {
   // V pairs of a thread as 16-byte accesses need rows, heads and halves on 16 bytes; 8-byte ones and single
-  // elements take the others (4096 rows of 32 heads: 12.3, 12.9 and 22.4 us)
+  // elements take the others (4096 rows of 32 heads in place: 9.3, 11.1 and 20.0 us)
   const uint64_t al = (uint64_t)a.x | (uint64_t)a.out | (uint64_t)(2 * (a.ldx | a.ldo | a.hs)) |
                       (uint64_t)(inter ? 0 : 2 * a.pairs);
 #define ROPE_LAUNCH(V)                                                             \
