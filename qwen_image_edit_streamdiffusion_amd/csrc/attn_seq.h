@@ -145,7 +145,7 @@ __device__ __forceinline__ float quad_sum(float v) {
 // After a row's maximum has moved: is some row's largest logit so far from 0 that fma(score, c, -(maximum c)), where
 // one product is rounded and the other is not, is off by more than 2^-12 (half a unit of 4096)? At 1e10 it would be
 // hundreds where it should be 0. All later tiles of such a wave come here and subtract the maximum from the scores
-// themselves (mscale 0: not a second time). Costs the first tile: 0.4 % of the mean call, 0.3 us of a short one.
+// themselves (mscale 0: not a second time). Costs 0.2 % of the mean call, 5 % of the worst (7 x 45 new tokens over 400).
 constexpr float kFar = 4096.f;
 __device__ __forceinline__ bool seq_far(const SeqArgs& a, float m_run, float& above, float& mscale) {
   const bool far = __any(fabsf(m_run * a.c) > kFar && m_run > a.low);

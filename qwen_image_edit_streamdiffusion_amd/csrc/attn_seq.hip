@@ -349,19 +349,19 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
 // longest cache that a table can hold (packed sequences: their mean length). Rows are those of one kv
 // head, tokens * G; a group is a (row block, kv head). Times in us (device, median), bf16, head_dim 128, 28 heads
 // over 4 unless said, the other side in brackets.
-//   few rows (attn_seq_few), 16-row blocks: up to 256 groups with eight waves each (one prompt of 100 tokens 5.8
-//     [6.9 in 64-row blocks]), up to 512 with four, two a CU (one prompt of 200: 7.7 [9.9 with eight, 8.2 in 64-row
-//     blocks]; of 280: 8.8 [9.3]; past it, one of 300: 10.0 in 64-row blocks [11.2]), and more than that over up to 1500
-//     keys (80 tokens of 24 heads over 24, caches of 20, 300 and 1000: 16, 49 and 171 [26, 59 and 171 with eight]; over
-//     8000, eight and four are level at 1300). 32-row blocks over more than 256 keys where 16-row ones would be more than
-//     256 (200 new tokens over 1000: 13.8 [16.4 in 16-row, 25.9 in 64-row blocks]; 10 x 20 over 300, 16 heads of 80, 7.7
-//     [9.6]), or where a cache is read again for each 16 rows and that takes longer than the second half of a block: for
+//   few rows (attn_seq_few), 16-row blocks: up to 256 groups with eight waves each (one prompt of 100 tokens 5.9
+//     [6.9 in 64-row blocks, 5.5 with four]), up to 512 with four, two a CU (one prompt of 200: 7.1 [9.9 with eight, 8.1
+//     in 64-row blocks]; of 280: 8.2 [9.3]; past it, one of 300: 10.0 in 64-row blocks [10.4]), and more than that over up
+//     to 1500 keys (80 tokens of 24 heads over 24, caches of 20, 300 and 1000: 15, 47 and 171 [26, 59 and 172 with eight];
+//     over 2000 and 8000: 333 and 1284 with eight [335 and 1291]). 32-row blocks over more than 256 keys where 16-row ones
+//     would be more than 256 (200 new tokens over 1000: 14.0 [15.3 in 16-row, 26.0 in 64-row blocks]; 10 x 20 over 300, 16
+//     heads of 80, 7.7 [8.9]; over 400 the 200 would take 9.2 in 16-row ones [10.6]), or where a cache is read again for each 16 rows and that takes longer than the second half of a block: for
 //     17 .. 32 rows a sequence from groups * keys = 6e4 on (3 new tokens over 6000 keys of one sequence 10.8 in 16-row
 //     blocks [12.5], over 20000 17.7 in 32-row ones [21.5]; 4 over 20000 of 16 sequences 138 [194]), for more rows from 4e5
 //     (8 over 20000 of one sequence: 21.0 in 16-row blocks [22.8]), and up to 1.5e6 against larger blocks (70 over 20000:
 //     68 [94 in 64-row ones]; 100: 79 in 256-row ones [128]).
 //   64-row blocks (attn_seq): shorter packed sequences (16 prompts of 400: 43 [53 in 256-row blocks]; from 200 groups
-//     on very short ones, 16 x 30, 16 heads of 80: 4.7 [6.2 in 16-row blocks]), a short
+//     on very short ones, 16 x 30, 16 heads of 80: 4.7 [5.9 in 16-row blocks]), a short
 //     cache's many rows (16 x 100 new tokens over 300: 19.5 [22.5 in 256-row blocks]), and 33 .. 64 rows of a sequence
 //     over a long one where 32-row ones are more than 3e5 groups * keys (3 x 8 new tokens over 20000: 31 [59]; 16 x 8 135
 //     [203]).
