@@ -369,8 +369,8 @@ __global__ void __launch_bounds__(256) attn_seq_join_kernel(SeqArgs a) {
 //     blocks]; 4 x 650, 182: 29 in 64-row ones [31]), their rounds of 256 are two thirds full (2 x 1600, 350: 49 [55]; 2 x
 //     1371, 300: level at 48), and the mean length is at least
 //       head_dim      causal, shared heads          causal, not shared             full
-//       97 .. 128     1000 (10 x 1000 107 [109],    2300 (24, 4 x 2500 189 [204],  900 (4 x 900 65 [69],
-//                     8 x 1300 129 [135],           4 x 1800 152 [123])            4 x 700 52 [45])
+//       97 .. 128     1000 (10 x 1000 107 [109],    2300 (24, 4 x 2500 189 [204],  800 (32 over 8, 29 of 570 .. 1084
+//                     8 x 1300 129 [135],           4 x 1800 152 [123])            466 [491]; 4 x 700 52 [45])
 //                     8 x 900 80 [76])
 //       65 .. 96      1800 (16 over 2, 8 x 1800     2300 (16, 4 x 2500 113 [117],  900 (16, 8 x 900 61 [64],
 //                     113 [119], 8 x 1400 79 [78])  4 x 2000 91 [81])              8 x 800 54 [50])
@@ -397,7 +397,7 @@ SeqPlan seq_plan(int tokens, int seqs, int heads, int kv_heads, int head_dim, bo
   const int few16 = r16 <= 256 ? 8 : 4;
   // from what length on 256-row blocks pay, and how full their rounds of 256 are
   const bool shared = heads > kv_heads;
-  const double longest = head_dim > 64 ? (!causal ? 900 : !shared ? 2300 : head_dim > 96 ? 1000 : 1800)
+  const double longest = head_dim > 64 ? (!causal ? (head_dim > 96 ? 800 : 900) : !shared ? 2300 : head_dim > 96 ? 1000 : 1800)
                          : shared      ? (causal ? 3500 : 1500)
                                        : (causal ? 6500 : 2700);
   const double rounds = ceil(g256 / 256), pad = ceil(per / kPPRows) * kPPRows / per;
